@@ -530,6 +530,99 @@ int rwkv7_fused_lm_head_ce_partial(const rwkv7_tensor *x, const rwkv7_tensor *we
 int rwkv7_lm_head_ce_finalize(const rwkv7_tensor *partials_all, const rwkv7_tensor *targets,
                               rwkv7_tensor *lse, rwkv7_tensor *loss, rwkv7_stream stream);
 
+/* ------------------------------------------------------ linear attention -- */
+/*
+ * Linear attention with one decay per head.  No counterpart in the reference; the state has the layout of the WKV7 entries.
+ * Per (b,h), d = exp(log_decay[h]), S[i][j] (i value row, j key column), t = 0 .. len_b - 1:
+ *   S[i][j] = d S[i][j] + value[b,t,h,i] key[b,t,h,j];   output[b,t,h,i] = sum_j S[i][j] query[b,t,h,j].
+ * query, key, value and output are [B,T,H,N], all F32 or all BF16, N = 32, 64 or 128; T >= 1.  log_decay is [H] F32 (a model
+ * has values up to 0; larger ones are computed as the formula says), states are [B,H,N,N] F32; sums and the carried state are
+ * fp32.  initial_state may be NULL (zero) and next_state NULL (not wanted); they may be the same tensor.  No scale is applied
+ * to the queries.
+ * context_lens ([B] I32, may be NULL) gives each sequence of a padded batch its length, 0 .. T (smaller values count as 0, larger
+ * ones as T): the tokens behind it are not read into anything, their output is zero, and the final state is the one at the length.
+ * The workspace lets a call of few chains work on several parts of a sequence at once; a smaller one than the call below names, or
+ * NULL, makes fewer parts of it (results differ in the last bits).  It must start on 16 bytes.
+ */
+size_t rwkv7_linear_attention_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t N, int32_t dtype);
+int rwkv7_fused_linear_attention(const rwkv7_tensor *initial_state, const rwkv7_tensor *query, const rwkv7_tensor *key,
+                                 const rwkv7_tensor *value, const rwkv7_tensor *log_decay, const rwkv7_tensor *context_lens,
+                                 rwkv7_tensor *output, rwkv7_tensor *next_state, void *workspace, size_t workspace_bytes,
+                                 rwkv7_stream stream);
+/*
+ * Its gradients, from the gradient of the output and of the final state (NULL: zero).  initial_state is the state the forward pass
+ * started from (NULL: zero); initial_state_grad may be NULL.  The decay is a constant of the model and has no gradient.  Gradients
+ * of tokens behind their sequence's length are zero.  The gradients may not share memory with any input.
+ */
+size_t rwkv7_linear_attention_backward_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t N, int32_t dtype);
+int rwkv7_fused_linear_attention_backward(const rwkv7_tensor *initial_state, const rwkv7_tensor *query, const rwkv7_tensor *key,
+                                          const rwkv7_tensor *value, const rwkv7_tensor *log_decay,
+                                          const rwkv7_tensor *context_lens, const rwkv7_tensor *output_grad,
+                                          const rwkv7_tensor *next_state_grad, rwkv7_tensor *query_grad, rwkv7_tensor *key_grad,
+                                          rwkv7_tensor *value_grad, rwkv7_tensor *initial_state_grad, void *workspace,
+                                          size_t workspace_bytes, rwkv7_stream stream);
+
+/* ---------------------------------------------------------- residual norm -- */
+/*
+ * What stands between two blocks of a cell, for rows of C channels ([B,T,C], C <= 8192).  No counterpart in the reference, whose
+ * cells (cells/causal.rs:213-248) are the case without post norm, gate and scale:
+ *   u = norm_post(block_output)   (block_output itself without post_gamma)
+ *   next_residual = residual + residual_scale * (gate * u)
+ *   normed = norm_pre(next_residual)   (of the sum before it is rounded)
+ *   norm(v) = (v - mean v) / sqrt(var v + epsilon) * gamma + beta over the C channels (biased variance);
+ *   RWKV7_NORM_RMS: v / sqrt(mean v^2 + epsilon) * gamma + beta.
+ * NULL leaves a part out: gate, residual_scale (ones), the betas (zeros), post_gamma (no norm after the block), pre_gamma with
+ * normed (no norm of the sum), block_output with everything that belongs to it and next_residual (normed = norm_pre(residual)).
+ * Parameters hold C elements; all tensors F32 or all BF16, arithmetic in fp32, each result rounded once.  next_residual and
+ * normed may each be the same tensor as residual, block_output or gate, but not as one another.
+ */
+typedef enum rwkv7_norm_kind { RWKV7_NORM_LAYER = 0, RWKV7_NORM_RMS = 1 } rwkv7_norm_kind;
+int rwkv7_fused_residual_norm(const rwkv7_tensor *residual, const rwkv7_tensor *block_output, const rwkv7_tensor *gate,
+                              const rwkv7_tensor *residual_scale, const rwkv7_tensor *post_gamma, const rwkv7_tensor *post_beta,
+                              const rwkv7_tensor *pre_gamma, const rwkv7_tensor *pre_beta, int32_t kind, double epsilon,
+                              rwkv7_tensor *next_residual, rwkv7_tensor *normed, rwkv7_stream stream);
+/*
+ * Its gradients, from those of next_residual (NULL: zero) and normed (given if and only if pre_gamma is).  `grads` are in the order
+ * residual, block_output, gate, residual_scale, post_gamma, post_beta, pre_gamma, pre_beta, one for each tensor that was
+ * given and NULL for the rest; those of parameters are summed over the rows in fp32, in an order that depends on the shape and the
+ * device alone.  The gradients may not share memory with any input.  The workspace must start on 16 bytes; its size depends on the
+ * SM count of the calling thread's current device.
+ */
+size_t rwkv7_residual_norm_backward_workspace_bytes(int64_t rows, int64_t C);
+int rwkv7_fused_residual_norm_backward(const rwkv7_tensor *residual, const rwkv7_tensor *block_output, const rwkv7_tensor *gate,
+                                       const rwkv7_tensor *residual_scale, const rwkv7_tensor *post_gamma,
+                                       const rwkv7_tensor *post_beta, const rwkv7_tensor *pre_gamma, const rwkv7_tensor *pre_beta,
+                                       int32_t kind, double epsilon, const rwkv7_tensor *next_residual_grad,
+                                       const rwkv7_tensor *normed_grad, rwkv7_tensor *const grads[8], void *workspace,
+                                       size_t workspace_bytes, rwkv7_stream stream);
+
+/* ------------------------------------------------------------ beam search -- */
+/*
+ * One step of B beam searches of I beams each (I <= 32), K of which go on (K <= 32, K <= I * V); no counterpart in the reference.
+ * Candidate (i, t) of search b is token t behind beam i, with
+ *   scores[b,i] + logits[b,i,t] - log sum_u exp(logits[b,i,u]);
+ * next_scores, parents (i) and tokens (t), all [B,K], are the K largest in falling order, ties by the lowest i * V + t.  Scores are
+ * compared in 64 bits (next_scores are F32); the sums of exponentials are fp32.
+ * logits [B,I,V] F32 or BF16, scores [B,I] F32.  A NaN among them counts as -inf, +inf as the largest finite number; a beam without
+ * any logit above -inf has candidates of -inf only, which are chosen, by their index, when nothing else is left.  finished ([B,I]
+ * I32, may be NULL): a beam whose entry is not zero has the candidate pad_token at its own score, and -inf for the rest.
+ * workspace: rwkv7_beam_select_workspace_bytes, on 16 bytes.
+ */
+size_t rwkv7_beam_select_workspace_bytes(int64_t B, int64_t I, int64_t V, int64_t K);
+int rwkv7_beam_select(const rwkv7_tensor *logits, const rwkv7_tensor *scores, const rwkv7_tensor *finished, int64_t pad_token,
+                      rwkv7_tensor *next_scores, rwkv7_tensor *parents, rwkv7_tensor *tokens, void *workspace,
+                      size_t workspace_bytes, rwkv7_stream stream);
+/*
+ * Moves the recurrent states of B searches to the beams that go on: with rows (the first axis) of I beams a search in, K out,
+ *   out[b * K + j] = states[b * I + parents[b,j]]
+ * for n tensors of any types and shapes behind the first axis, B * I rows each; parents is [B,K] I32 or I64, I and K <= 32.
+ * out NULL: in place (I == K), where rows that keep their place are not touched.  Otherwise n tensors like the states but of B * K
+ * rows.  No two tensors of a call may share memory.  A parent outside 0 .. I-1 leaves its row as it was and is reported as
+ * RWKV7_ERR_BAD_INDEX by rwkv7_read_device_status.
+ */
+int rwkv7_beam_reorder(const rwkv7_tensor *const *states, int32_t n, const rwkv7_tensor *parents, rwkv7_tensor *const *out,
+                       rwkv7_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

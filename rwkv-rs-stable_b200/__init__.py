@@ -592,3 +592,198 @@ def lm_head_ce_finalize(partials_all: torch.Tensor, targets: torch.Tensor):
 def lm_head_ce(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor):
     """Single-GPU fused LM-head cross entropy: per-row ``(lse, loss)``."""
     return (_native or native()).lm_head_ce(x, weight, targets)
+
+
+# ---------------------------------------------------------- linear attention --
+
+
+@dataclass
+class LinearAttentionForwardInputs:
+    """``query``, ``key``, ``value`` ``[batch, context_len, num_heads, head_size]`` (F32 or BF16, head size 32, 64 or 128),
+    ``log_decay`` ``[num_heads]`` F32 and, for a padded batch, ``context_lens`` ``[batch]`` int32."""
+
+    query: torch.Tensor
+    key: torch.Tensor
+    value: torch.Tensor
+    log_decay: torch.Tensor
+    context_lens: Optional[torch.Tensor] = None
+
+    def five(self):
+        return self.query, self.key, self.value, self.log_decay, self.context_lens
+
+
+@dataclass
+class LinearAttentionForwardOutput:
+    output: torch.Tensor
+    next_state: Optional[torch.Tensor]
+
+
+def linear_attention_custom(inputs: LinearAttentionForwardInputs, initial_state: Optional[torch.Tensor] = None, *,
+                            want_state: bool = True, next_state: Optional[torch.Tensor] = None,
+                            output: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None
+                            ) -> LinearAttentionForwardOutput:
+    """``rwkv7_fused_linear_attention``: ``S <- exp(log_decay) S + v k^T``, ``y = S q`` over every sequence, from
+    ``initial_state`` ``[B,H,N,N]`` F32 (zero when omitted).  One token is a decode step; ``next_state`` may be the same tensor as
+    ``initial_state``.  ``workspace``: a uint8 tensor of :func:`linear_attention_workspace_bytes`; allocated here when omitted."""
+    y, s = (_native or native()).linear_attention(initial_state, *inputs.five(), want_state or next_state is not None, next_state, output,
+                                                  workspace)
+    return LinearAttentionForwardOutput(output=y, next_state=s)
+
+
+linear_attention = linear_attention_custom
+
+
+def linear_attention_workspace_bytes(B: int, T: int, H: int, N: int, dtype: torch.dtype, *, backward: bool = False) -> int:
+    """``rwkv7_linear_attention_workspace_bytes`` (``backward``: of the backward pass) for the current device."""
+    fn = lib().rwkv7_linear_attention_backward_workspace_bytes if backward else lib().rwkv7_linear_attention_workspace_bytes
+    fn.restype = ctypes.c_size_t
+    return int(fn(*(ctypes.c_int64(x) for x in (B, T, H, N)), ctypes.c_int32(_DTYPES.get(dtype, -1))))
+
+
+def linear_attention_backward(inputs: LinearAttentionForwardInputs, output_grad: torch.Tensor,
+                              next_state_grad: Optional[torch.Tensor] = None, *, initial_state: Optional[torch.Tensor] = None,
+                              want_state_grad: bool = True, workspace: Optional[torch.Tensor] = None):
+    """``rwkv7_fused_linear_attention_backward``: ``((query, key, value gradient), initial_state_grad or None)``.  The decay is a
+    constant and has no gradient."""
+    dq, dk, dv, ds = (_native or native()).linear_attention_backward(initial_state, *inputs.five(), output_grad, next_state_grad,
+                                                                     want_state_grad, workspace)
+    return (dq, dk, dv), ds
+
+
+class _LinearAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, context_lens, s0):
+        ctx.set_materialize_grads(False)
+        out = linear_attention_custom(LinearAttentionForwardInputs(q, k, v, log_decay, context_lens), s0)
+        ctx.save_for_backward(q, k, v, log_decay, context_lens, s0)
+        return out.output, out.next_state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, ds):
+        q, k, v, log_decay, context_lens, s0 = ctx.saved_tensors
+        dy = torch.zeros_like(q) if dy is None else dy.contiguous()
+        grads, ds0 = linear_attention_backward(LinearAttentionForwardInputs(q, k, v, log_decay, context_lens), dy,
+                                               None if ds is None else ds.contiguous(), initial_state=s0,
+                                               want_state_grad=ctx.needs_input_grad[5])
+        return (*grads, None, None, ds0)
+
+
+def linear_attention_autograd(initial_state: Optional[torch.Tensor], inputs: LinearAttentionForwardInputs):
+    """Differentiable linear attention: ``(output, next_state)`` with gradients to query, key, value and the initial state."""
+    if inputs.log_decay.requires_grad:
+        raise KernelInputsError(8, "Unsupported: linear_attention has no gradient for log_decay; pass it detached")
+    return _LinearAttentionFunction.apply(*(t.contiguous() for t in (inputs.query, inputs.key, inputs.value)), inputs.log_decay,
+                                          inputs.context_lens, initial_state)
+
+
+# ------------------------------------------------------------- residual norm --
+
+NORM_KINDS = {"layer": 0, "rms": 1}
+
+
+@dataclass
+class ResidualNormForwardInputs:
+    """What stands between two blocks of a cell (``rwkv7_fused_residual_norm``): ``residual``, ``block_output``, ``gate``
+    ``[batch, context_len, channels]`` and parameters of ``channels`` elements; what is None is left out."""
+
+    residual: torch.Tensor
+    block_output: Optional[torch.Tensor] = None
+    gate: Optional[torch.Tensor] = None
+    residual_scale: Optional[torch.Tensor] = None
+    post_gamma: Optional[torch.Tensor] = None
+    post_beta: Optional[torch.Tensor] = None
+    pre_gamma: Optional[torch.Tensor] = None
+    pre_beta: Optional[torch.Tensor] = None
+    kind: str = "layer"
+    epsilon: float = 1e-5
+
+    def eight(self):
+        return (self.residual, self.block_output, self.gate, self.residual_scale, self.post_gamma, self.post_beta, self.pre_gamma,
+                self.pre_beta)
+
+    def kind_code(self) -> int:
+        if self.kind not in NORM_KINDS:
+            raise KernelInputsError(14, f"BadArgument: norm kind {self.kind!r}, expected 'layer' or 'rms'")
+        return NORM_KINDS[self.kind]
+
+
+@dataclass
+class ResidualNormForwardOutput:
+    next_residual: Optional[torch.Tensor]   # None without a block output
+    normed: Optional[torch.Tensor]          # None without pre_gamma
+
+
+def residual_norm_custom(inputs: ResidualNormForwardInputs, *, next_residual: Optional[torch.Tensor] = None,
+                         normed: Optional[torch.Tensor] = None) -> ResidualNormForwardOutput:
+    """``next_residual = residual + residual_scale (gate norm_post(block_output))`` and ``normed = norm_pre(next_residual)`` in one
+    pass.  ``next_residual`` may be the same tensor as ``residual`` (an update in place)."""
+    x, z = (_native or native()).residual_norm(*inputs.eight(), inputs.kind_code(), inputs.epsilon, next_residual, normed)
+    return ResidualNormForwardOutput(next_residual=x, normed=z)
+
+
+residual_norm = residual_norm_custom
+
+
+def residual_norm_backward(inputs: ResidualNormForwardInputs, next_residual_grad: Optional[torch.Tensor] = None,
+                           normed_grad: Optional[torch.Tensor] = None, *, workspace: Optional[torch.Tensor] = None):
+    """``rwkv7_fused_residual_norm_backward``: the gradients of the eight tensors of ``inputs``, in their order, None for those that
+    were not given.  ``inputs.residual`` is the residual as it was before the forward pass."""
+    return (_native or native()).residual_norm_backward(*inputs.eight(), inputs.kind_code(), inputs.epsilon, next_residual_grad,
+                                                        normed_grad, workspace)
+
+
+class _ResidualNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, kind, epsilon, *eight):
+        ctx.set_materialize_grads(False)
+        ctx.kind, ctx.epsilon = kind, epsilon
+        ctx.save_for_backward(*eight)
+        out = residual_norm_custom(ResidualNormForwardInputs(*eight, kind=kind, epsilon=epsilon))
+        return out.next_residual, out.normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dnext, dnormed):
+        eight = ctx.saved_tensors
+        if eight[6] is not None:
+            dnormed = torch.zeros_like(eight[0]) if dnormed is None else dnormed.contiguous()
+        grads = residual_norm_backward(ResidualNormForwardInputs(*eight, kind=ctx.kind, epsilon=ctx.epsilon),
+                                       None if dnext is None else dnext.contiguous(), dnormed)
+        return (None, None, *grads)
+
+
+def residual_norm_autograd(inputs: ResidualNormForwardInputs):
+    """Differentiable :func:`residual_norm_custom`: ``(next_residual or None, normed or None)``."""
+    return _ResidualNormFunction.apply(inputs.kind, inputs.epsilon, *(None if t is None else t.contiguous() for t in inputs.eight()))
+
+
+# --------------------------------------------------------------- beam search --
+
+
+@dataclass
+class BeamSelectOutput:
+    scores: torch.Tensor    # [B, num_beams] F32, falling
+    parents: torch.Tensor   # [B, num_beams] int32: the beam each goes on from
+    tokens: torch.Tensor    # [B, num_beams] int32
+
+
+def beam_select_custom(logits: torch.Tensor, scores: torch.Tensor, num_beams: int, *, finished: Optional[torch.Tensor] = None,
+                       pad_token: int = 0, workspace: Optional[torch.Tensor] = None) -> BeamSelectOutput:
+    """``rwkv7_beam_select``: the ``num_beams`` best of ``scores[b,i] + log_softmax(logits[b,i])[t]`` over beams and vocabulary,
+    ties by the lowest ``i * V + t``.  ``logits`` ``[B, beams, V]`` F32 or BF16, ``scores`` ``[B, beams]`` F32; a beam whose entry of
+    ``finished`` ``[B, beams]`` int32 is not zero goes on with ``pad_token`` at its own score."""
+    return BeamSelectOutput(*(_native or native()).beam_select(logits, scores, num_beams, finished, pad_token, workspace))
+
+
+beam_select = beam_select_custom
+
+
+def beam_reorder_custom(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None):
+    """``rwkv7_beam_reorder``: row ``b * num_beams + j`` of every result is row ``b * beams + parents[b,j]`` of its state, for
+    tensors ``[B * beams, ...]`` of any type and shape (WKV7 and linear-attention states, shifted tokens).  In place, where rows
+    that stay are not touched, or into ``out``.  Returns the tensors written."""
+    return (_native or native()).beam_reorder(list(states), parents, None if out is None else list(out))
+
+
+beam_reorder = beam_reorder_custom

@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cstdint>
 
+#include "abi_common.h"
 #include "check.h"
 #include "kernels.h"
 #include "rwkv7_b200.h"
@@ -17,52 +18,6 @@ namespace {
 
 std::atomic<int> g_wkv7_path{RWKV7_WKV7_AUTO};
 
-constexpr int kMaxDevices = 64;
-std::atomic<int> g_num_sms[kMaxDevices] = {};
-
-// Makes `device` current for the duration of a call and restores the caller's.  A thread's first call sets the device in any
-// case: until a thread has done something with its device it has no current context, and a tensor map cannot be encoded.
-class DeviceGuard {
-   public:
-    explicit DeviceGuard(int device) {
-        static thread_local int bound = -1;
-        err_ = cudaGetDevice(&prev_);
-        if (err_ == cudaSuccess && (prev_ != device || bound != device)) {
-            err_ = cudaSetDevice(device);
-            switched_ = err_ == cudaSuccess && prev_ != device;
-            if (err_ == cudaSuccess) bound = device;
-        }
-    }
-    ~DeviceGuard() {
-        if (switched_) cudaSetDevice(prev_);
-    }
-    cudaError_t error() const { return err_; }
-
-   private:
-    int prev_ = 0;
-    bool switched_ = false;
-    cudaError_t err_ = cudaSuccess;
-};
-
-int cuda_fail(const char *what, int err) {
-    return fail(RWKV7_ERR_CUDA, "CudaError: %s: %s", what, cudaGetErrorString((cudaError_t)err));
-}
-
-int num_sms(int device, int *out) {
-    if (device < 0 || device >= kMaxDevices)
-        return fail(RWKV7_ERR_BAD_ARGUMENT, "BadArgument: device ordinal %d out of range", device);
-    int v = g_num_sms[device].load(std::memory_order_relaxed);
-    if (v == 0) {
-        cudaError_t e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device);
-        if (e != cudaSuccess) return cuda_fail("cudaDeviceGetAttribute", (int)e);
-        g_num_sms[device].store(v, std::memory_order_relaxed);
-    }
-    *out = v;
-    return RWKV7_OK;
-}
-
-bool float_dtype_supported(int32_t dt) { return dt == RWKV7_F32 || dt == RWKV7_BF16; }
-
 // Shortest sequences the automatic choice gives to the two-kernel prefill.  bf16: one chunk; up to kSplitTiersTokens the scan
 // recomputes a flagged chain itself (token by token), so that a short call is two launches, beyond that the chain goes
 // through the tf32 chunked kernel, which is faster from about there.  fp32: the scan's fp16 operands are less precise
@@ -71,11 +26,6 @@ constexpr int64_t kSplitMinTokens = 64;
 constexpr int64_t kSplitTiersTokens = 512;
 constexpr int64_t kSplitMinTokensF32 = 512;
 int64_t split_min_tokens(bool bf16) { return bf16 ? kSplitMinTokens : kSplitMinTokensF32; }
-
-#define RWKV7_TRY(expr)                 \
-    do {                                \
-        if (int st_ = (expr)) return st_; \
-    } while (0)
 
 // check_wkv7_sequence_inputs (wkv7/io.rs:175-241) + the contiguity assertions of
 // the CubeBackend impl (wkv7/mod.rs:56-76).  `chunk_len == 16` and

@@ -222,4 +222,73 @@ int launch_lm_head_ce_finalize(const float *partials_all, int num_shards, const 
                                int targets_dtype, float *lse, float *loss, int64_t R,
                                cudaStream_t stream);
 
+// One pass of linear attention over sequences [B,T,H,N] (linear_attention.cu has the recurrence): y from (a, b, c), forwards or
+// reversed.  States are [B,H,N,N]: row of c, column of b; `s_in_transposed`: what is read is laid out the other way round.
+struct LinearAttentionPass {
+    const void *a, *b, *c;     // bf16 or f32
+    void *y;
+    const float *log_decay;    // [H]
+    const int *lens;           // [B] or null (all T)
+    const float *s_in;         // or null (zero)
+    float *s_out;              // or null; may be s_in
+    int64_t B, T, H, N;
+    bool s_in_transposed, reversed, bf16;
+    int device, num_sms;
+};
+bool linear_attention_supported(int64_t N);
+int launch_linear_attention(const LinearAttentionPass &p, cudaStream_t stream);
+
+// The norms before and after a block with its gate and residual scale; rows of C channels, parameters [C].
+struct ResidualNormArgs {
+    const void *residual, *block_output, *gate;                              // [rows,C]; the last two may be null
+    const void *residual_scale, *post_gamma, *post_beta, *pre_gamma, *pre_beta;   // [C] or null
+    void *next_residual, *normed;                                            // [rows,C]; null: not wanted
+    float epsilon;
+    int64_t rows, C;
+    bool layer;   // else rms
+    bool bf16;
+    int num_sms;
+};
+struct ResidualNormBackwardArgs {
+    ResidualNormArgs f;                                    // (its outputs are not used)
+    const void *next_residual_grad, *normed_grad;          // [rows,C] or null
+    void *residual_grad, *block_output_grad, *gate_grad;   // [rows,C]
+    void *param_grads[5];                                  // [C] or null: scale, post gamma, post beta, pre gamma, pre beta
+};
+int64_t residual_norm_max_channels();
+int launch_residual_norm(const ResidualNormArgs &p, cudaStream_t stream);
+size_t residual_norm_backward_workspace_bytes(int64_t rows, int64_t C, int num_sms);
+int launch_residual_norm_backward(const ResidualNormBackwardArgs &p, void *workspace, cudaStream_t stream);
+
+// Beam search: B searches of I beams over V tokens, K chosen.
+struct BeamSelectArgs {
+    const void *logits;      // [B,I,V]
+    const float *scores;     // [B,I]
+    const int *finished;     // [B,I] or null
+    float *next_scores;      // [B,K]
+    int *parents, *tokens;   // [B,K]
+    int64_t B, V, pad_token;
+    int I, K;
+    bool bf16;
+    int num_sms;
+};
+size_t beam_select_workspace_bytes(int64_t B, int64_t I, int64_t K);
+int launch_beam_select(const BeamSelectArgs &p, void *workspace, cudaStream_t stream);
+constexpr int kMaxReordered = 48;   // tensors per launch
+struct BeamReorderArgs {
+    struct Item {
+        const void *from;   // B*I rows
+        void *to;           // B*K rows; `from` itself: in place (I == K)
+        int64_t row_bytes;
+    } tensors[kMaxReordered];
+    int n;
+    const void *parents;   // [B,K] i32 or i64
+    bool parents_i64;
+    int64_t B;
+    int I, K;
+    int *status;
+    int num_sms;
+};
+int launch_beam_reorder(const BeamReorderArgs &p, cudaStream_t stream);
+
 }  // namespace rwkv7

@@ -13,12 +13,16 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <memory>
+#include <vector>
 
 #include "rwkv7_b200.h"
 
@@ -37,7 +41,11 @@ namespace {
     X(rwkv7_fused_token_shift_diff_into)                                                                         \
     X(rwkv7_fused_weight_prepare) X(rwkv7_fused_gated_readout) X(rwkv7_channel_mixer_workspace_bytes)            \
     X(rwkv7_fused_channel_mixer) X(rwkv7_lm_head_ce_workspace_bytes) X(rwkv7_fused_lm_head_ce_partial)           \
-    X(rwkv7_lm_head_ce_finalize)
+    X(rwkv7_lm_head_ce_finalize) X(rwkv7_linear_attention_workspace_bytes) X(rwkv7_fused_linear_attention)       \
+    X(rwkv7_linear_attention_backward_workspace_bytes) X(rwkv7_fused_linear_attention_backward)                  \
+    X(rwkv7_fused_residual_norm) X(rwkv7_residual_norm_backward_workspace_bytes)                                 \
+    X(rwkv7_fused_residual_norm_backward) X(rwkv7_beam_select_workspace_bytes) X(rwkv7_beam_select)              \
+    X(rwkv7_beam_reorder)
 
 struct Abi {
 #define RWKV7_FIELD(name) decltype(&::name) name = nullptr;
@@ -602,6 +610,163 @@ PyObject *lm_head_ce(PyObject *const *a) {
     return lm_head_finalize_of(p.unsqueeze(0), a[2]);
 }
 
+// linear_attention(initial_state|None, query, key, value, log_decay, context_lens|None, want_state, next_state|None, output|None,
+//                  workspace|None) -> (output, next_state|None)
+PyObject *linear_attention(PyObject *const *a) {
+    Desc s0(a[0]), qkv[3], decay(a[4]), lens(a[5]), sd;
+    for (int i = 0; i < 3; ++i) qkv[i].set(a[1 + i]);
+    const at::Tensor &q = tensor(a[1]);
+    at::Tensor y_t, s_t;
+    if (a[8] == Py_None) y_t = like(q);
+    Desc yd(a[8] == Py_None ? y_t : tensor(a[8]));
+    const bool want_state = truth(a[6]);
+    Workspace ws;
+    if (q.dim() == 4) {
+        if (a[9] == Py_None) ws.allocate(abi.rwkv7_linear_attention_workspace_bytes(q.size(0), q.size(1), q.size(2), q.size(3), qkv[0].d.dtype), q);
+        if (want_state && a[7] == Py_None) s_t = empty({q.size(0), q.size(2), q.size(3), q.size(3)}, at::kFloat, q);
+    }
+    if (a[9] != Py_None) ws.given(a[9]);
+    if (want_state && a[7] != Py_None) sd.set(a[7]);
+    else if (s_t.defined()) sd.set(s_t);
+    const rwkv7_stream st = stream_of(q);
+    call([&] {
+        return abi.rwkv7_fused_linear_attention(s0.p, qkv[0].p, qkv[1].p, qkv[2].p, decay.p, lens.p, yd.p, sd.p, ws.ptr, ws.bytes, st);
+    });
+    return pair(given_or_wrapped(a[8], y_t), want_state ? given_or_wrapped(a[7], s_t) : Py_NewRef(Py_None));
+}
+
+// linear_attention_backward(initial_state|None, query, key, value, log_decay, context_lens|None, output_grad, next_state_grad|None,
+//                           want_state_grad, workspace|None) -> (query, key, value gradient, state gradient|None)
+PyObject *linear_attention_backward(PyObject *const *a) {
+    Desc s0(a[0]), qkv[3], decay(a[4]), lens(a[5]), dy(a[6]), ds(a[7]), gd[4];
+    for (int i = 0; i < 3; ++i) qkv[i].set(a[1 + i]);
+    const at::Tensor &q = tensor(a[1]);
+    at::Tensor grads[4];
+    for (int i = 0; i < 3; ++i) {
+        grads[i] = like(q);
+        gd[i].set(grads[i]);
+    }
+    Workspace ws;
+    if (q.dim() == 4) {
+        if (truth(a[8])) {
+            grads[3] = empty({q.size(0), q.size(2), q.size(3), q.size(3)}, at::kFloat, q);
+            gd[3].set(grads[3]);
+        }
+        if (a[9] == Py_None)
+            ws.allocate(abi.rwkv7_linear_attention_backward_workspace_bytes(q.size(0), q.size(1), q.size(2), q.size(3), qkv[0].d.dtype), q);
+    }
+    if (a[9] != Py_None) ws.given(a[9]);
+    const rwkv7_stream st = stream_of(q);
+    call([&] {
+        return abi.rwkv7_fused_linear_attention_backward(s0.p, qkv[0].p, qkv[1].p, qkv[2].p, decay.p, lens.p, dy.p, ds.p, gd[0].p, gd[1].p,
+                                                         gd[2].p, gd[3].p, ws.ptr, ws.bytes, st);
+    });
+    return tuple_of(grads, 4);
+}
+
+double number(PyObject *o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PythonError{};
+    return v;
+}
+
+// residual_norm(residual, block_output|None, gate|None, residual_scale|None, post_gamma|None, post_beta|None, pre_gamma|None,
+//               pre_beta|None, kind, epsilon, next_residual|None, normed|None) -> (next_residual|None, normed|None)
+PyObject *residual_norm(PyObject *const *a) {
+    Desc in[8], od[2];
+    for (int i = 0; i < 8; ++i) in[i].set(a[i]);
+    const at::Tensor &x = tensor(a[0]);
+    const int32_t kind = (int32_t)integer(a[8]);
+    const double eps = number(a[9]);
+    const bool wanted[2] = {in[1].p != nullptr, in[6].p != nullptr};
+    at::Tensor out[2];
+    for (int i = 0; i < 2; ++i) {
+        if (a[10 + i] != Py_None) od[i].set(a[10 + i]);
+        else if (wanted[i]) {
+            out[i] = like(x);
+            od[i].set(out[i]);
+        }
+    }
+    const rwkv7_stream st = stream_of(x);
+    call([&] {
+        return abi.rwkv7_fused_residual_norm(in[0].p, in[1].p, in[2].p, in[3].p, in[4].p, in[5].p, in[6].p, in[7].p, kind, eps, od[0].p, od[1].p, st);
+    });
+    PyObject *r[2];
+    for (int i = 0; i < 2; ++i) r[i] = wanted[i] ? given_or_wrapped(a[10 + i], out[i]) : Py_NewRef(Py_None);
+    return pair(r[0], r[1]);
+}
+
+// residual_norm_backward(the first ten as residual_norm, next_residual_grad|None, normed_grad|None, workspace|None)
+//   -> eight gradients, None for what was not given
+PyObject *residual_norm_backward(PyObject *const *a) {
+    Desc in[8], dnext(a[10]), dnormed(a[11]), gd[8];
+    at::Tensor grads[8];
+    rwkv7_tensor *gp[8];
+    for (int i = 0; i < 8; ++i) {
+        in[i].set(a[i]);
+        if (in[i].p) {
+            grads[i] = like(tensor(a[i]));
+            gd[i].set(grads[i]);
+        }
+        gp[i] = gd[i].p;
+    }
+    const at::Tensor &x = tensor(a[0]);
+    const int32_t kind = (int32_t)integer(a[8]);
+    const double eps = number(a[9]);
+    Workspace ws;
+    if (a[12] != Py_None) ws.given(a[12]);
+    else if (x.dim() == 3) {
+        const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? std::make_optional(x.device()) : std::nullopt);
+        ws.allocate(abi.rwkv7_residual_norm_backward_workspace_bytes(x.size(0) * x.size(1), x.size(2)), x);
+    }
+    const rwkv7_stream st = stream_of(x);
+    call([&] {
+        return abi.rwkv7_fused_residual_norm_backward(in[0].p, in[1].p, in[2].p, in[3].p, in[4].p, in[5].p, in[6].p, in[7].p, kind, eps, dnext.p,
+                                                      dnormed.p, gp, ws.ptr, ws.bytes, st);
+    });
+    return tuple_of(grads, 8);
+}
+
+// beam_select(logits, scores, num_beams, finished|None, pad_token, workspace|None) -> (scores, parents, tokens)
+PyObject *beam_select(PyObject *const *a) {
+    const at::Tensor &logits = tensor(a[0]);
+    Desc ld(logits), sd(a[1]), fd(a[3]);
+    const int64_t K = integer(a[2]), pad = integer(a[4]), B = logits.dim() > 0 ? logits.size(0) : 0;
+    if (K < 0) raise(PyExc_ValueError, "num_beams must not be negative");
+    const at::Tensor out[3] = {empty({B, K}, at::kFloat, logits), empty({B, K}, at::kInt, logits), empty({B, K}, at::kInt, logits)};
+    Desc od[3];
+    for (int i = 0; i < 3; ++i) od[i].set(out[i]);
+    Workspace ws;
+    if (a[5] != Py_None) ws.given(a[5]);
+    else if (logits.dim() == 3) ws.allocate(abi.rwkv7_beam_select_workspace_bytes(B, logits.size(1), logits.size(2), K), logits);
+    const rwkv7_stream st = stream_of(logits);
+    call([&] { return abi.rwkv7_beam_select(ld.p, sd.p, fd.p, pad, od[0].p, od[1].p, od[2].p, ws.ptr, ws.bytes, st); });
+    return tuple_of(out, 3);
+}
+
+// beam_reorder(list of states, parents, list of outputs|None)
+PyObject *beam_reorder(PyObject *const *a) {
+    if (!PyList_Check(a[0]) || (a[2] != Py_None && !PyList_Check(a[2]))) raise(PyExc_TypeError, "expected a list of tensors");
+    const Py_ssize_t n = PyList_GET_SIZE(a[0]);
+    if (a[2] != Py_None && PyList_GET_SIZE(a[2]) != n) raise(PyExc_ValueError, "as many outputs as states");
+    const at::Tensor &parents = tensor(a[1]);
+    Desc pd(parents);
+    const std::unique_ptr<Desc[]> sd(new Desc[n + 1]), od(new Desc[n + 1]);
+    std::vector<const rwkv7_tensor *> sp(n);
+    std::vector<rwkv7_tensor *> op(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        sd[i].set(tensor(PyList_GET_ITEM(a[0], i)));
+        sp[i] = sd[i].p;
+        if (a[2] != Py_None) {
+            od[i].set(tensor(PyList_GET_ITEM(a[2], i)));
+            op[i] = od[i].p;
+        }
+    }
+    const rwkv7_stream st = stream_of(parents);
+    call([&] { return abi.rwkv7_beam_reorder(sp.data(), (int32_t)n, pd.p, a[2] == Py_None ? nullptr : op.data(), st); });
+    return Py_NewRef(a[2] == Py_None ? a[0] : a[2]);
+}
+
 // ---- module ---------------------------------------------------------------------------------------
 
 // Checks the number of arguments and turns what is thrown below into a Python exception.
@@ -652,7 +817,8 @@ PyMethodDef methods[] = {
     RWKV7_METHOD(mix6, 7), RWKV7_METHOD(mix6_stacked, 7), RWKV7_METHOD(addcmul, 4), RWKV7_METHOD(addcmul5, 7),
     RWKV7_METHOD(token_shift_diff, 4), RWKV7_METHOD(weight_prepare, 9), RWKV7_METHOD(gated_readout, 10),
     RWKV7_METHOD(channel_mixer, 5), RWKV7_METHOD(lm_head_ce_partial, 4), RWKV7_METHOD(lm_head_ce_finalize, 2),
-    RWKV7_METHOD(lm_head_ce, 3),
+    RWKV7_METHOD(lm_head_ce, 3), RWKV7_METHOD(linear_attention, 10), RWKV7_METHOD(linear_attention_backward, 10),
+    RWKV7_METHOD(residual_norm, 12), RWKV7_METHOD(residual_norm_backward, 13), RWKV7_METHOD(beam_select, 6), RWKV7_METHOD(beam_reorder, 3),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "rwkv7_b200_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

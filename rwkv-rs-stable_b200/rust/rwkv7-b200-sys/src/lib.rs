@@ -51,6 +51,10 @@ pub const RWKV7_WKV7_SEQUENTIAL: c_int = 1;
 pub const RWKV7_WKV7_CHUNKED: c_int = 2;
 pub const RWKV7_WKV7_SPLIT: c_int = 3;
 
+// rwkv7_norm_kind
+pub const RWKV7_NORM_LAYER: i32 = 0;
+pub const RWKV7_NORM_RMS: i32 = 1;
+
 /// `device` value of a tensor descriptor that lives in pinned host memory.
 pub const RWKV7_HOST: i32 = -1;
 /// `flags` bit of `rwkv7_wkv7_statepass_host`: leave the caller's stream unjoined.
@@ -184,6 +188,34 @@ extern "C" {
     pub fn rwkv7_fused_lm_head_ce_partial(x: T, weight_shard: T, targets: T, vocab_offset: i64,
         partials: TM, workspace: *mut c_void, workspace_bytes: usize, stream: rwkv7_stream) -> c_int;
     pub fn rwkv7_lm_head_ce_finalize(partials_all: T, targets: T, lse: TM, loss: TM,
+        stream: rwkv7_stream) -> c_int;
+
+    // ---- linear attention with a decay per head
+    pub fn rwkv7_linear_attention_workspace_bytes(b: i64, t: i64, h: i64, n: i64, dtype: i32) -> usize;
+    pub fn rwkv7_fused_linear_attention(initial_state: T, query: T, key: T, value: T, log_decay: T,
+        context_lens: T, output: TM, next_state: TM, workspace: *mut c_void, workspace_bytes: usize,
+        stream: rwkv7_stream) -> c_int;
+    pub fn rwkv7_linear_attention_backward_workspace_bytes(b: i64, t: i64, h: i64, n: i64, dtype: i32) -> usize;
+    pub fn rwkv7_fused_linear_attention_backward(initial_state: T, query: T, key: T, value: T, log_decay: T,
+        context_lens: T, output_grad: T, next_state_grad: T, query_grad: TM, key_grad: TM, value_grad: TM,
+        initial_state_grad: TM, workspace: *mut c_void, workspace_bytes: usize, stream: rwkv7_stream) -> c_int;
+
+    // ---- norms before and after a block
+    pub fn rwkv7_fused_residual_norm(residual: T, block_output: T, gate: T, residual_scale: T, post_gamma: T,
+        post_beta: T, pre_gamma: T, pre_beta: T, kind: i32, epsilon: f64, next_residual: TM, normed: TM,
+        stream: rwkv7_stream) -> c_int;
+    pub fn rwkv7_residual_norm_backward_workspace_bytes(rows: i64, c: i64) -> usize;
+    pub fn rwkv7_fused_residual_norm_backward(residual: T, block_output: T, gate: T, residual_scale: T,
+        post_gamma: T, post_beta: T, pre_gamma: T, pre_beta: T, kind: i32, epsilon: f64,
+        next_residual_grad: T, normed_grad: T, grads: *const TM, workspace: *mut c_void,
+        workspace_bytes: usize, stream: rwkv7_stream) -> c_int;
+
+    // ---- beam search
+    pub fn rwkv7_beam_select_workspace_bytes(b: i64, i: i64, v: i64, k: i64) -> usize;
+    pub fn rwkv7_beam_select(logits: T, scores: T, finished: T, pad_token: i64, next_scores: TM,
+        parents: TM, tokens: TM, workspace: *mut c_void, workspace_bytes: usize,
+        stream: rwkv7_stream) -> c_int;
+    pub fn rwkv7_beam_reorder(states: *const T, n: i32, parents: T, out: *const TM,
         stream: rwkv7_stream) -> c_int;
 }
 
