@@ -104,13 +104,26 @@ int check_linear_attention(const TensorInfo &s0, const TensorInfo (&qkv)[3], con
     return RWKV7_OK;
 }
 
+size_t attention_workspace(int64_t B, int64_t T, int64_t H, int64_t N, int32_t dtype) {
+    LinearAttentionPass p{};
+    p.B = B; p.T = T; p.H = H; p.N = N;
+    p.bf16 = dtype == RWKV7_BF16;
+    p.num_sms = current_sms();
+    return B <= 0 || T <= 0 || H <= 0 || !float_dtype_supported(dtype) || !linear_attention_supported(N) ? 0 : linear_attention_workspace_bytes(p);
+}
+
 }  // namespace
 
 extern "C" {
 
-size_t rwkv7_linear_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int32_t) { return 0; }
+size_t rwkv7_linear_attention_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t N, int32_t dtype) {
+    return attention_workspace(B, T, H, N, dtype);
+}
 
-size_t rwkv7_linear_attention_backward_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int32_t) { return 0; }
+// (its passes use it in turn)
+size_t rwkv7_linear_attention_backward_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t N, int32_t dtype) {
+    return attention_workspace(B, T, H, N, dtype);
+}
 
 int rwkv7_fused_linear_attention(const rwkv7_tensor *s0_t, const rwkv7_tensor *q_t, const rwkv7_tensor *k_t, const rwkv7_tensor *v_t,
                                  const rwkv7_tensor *decay_t, const rwkv7_tensor *lens_t, rwkv7_tensor *y_t, rwkv7_tensor *s_t,
@@ -136,7 +149,7 @@ int rwkv7_fused_linear_attention(const rwkv7_tensor *s0_t, const rwkv7_tensor *q
     p.a = q_t->data; p.b = k_t->data; p.c = v_t->data; p.y = y_t->data;
     p.s_in = s0_t == nullptr ? nullptr : static_cast<const float *>(s0_t->data);
     p.s_out = s_t == nullptr ? nullptr : static_cast<float *>(s_t->data);
-    if (int e = launch_linear_attention(p, (cudaStream_t)stream)) return cuda_fail("linear_attention launch", e);
+    if (int e = launch_linear_attention(p, workspace, workspace_bytes, (cudaStream_t)stream)) return cuda_fail("linear_attention launch", e);
     return RWKV7_OK;
 }
 
@@ -176,7 +189,7 @@ int rwkv7_fused_linear_attention_backward(const rwkv7_tensor *s0_t, const rwkv7_
     dk.a = v_t->data; dk.b = dy_t->data; dk.c = q_t->data; dk.y = dk_t->data; dk.reversed = true;
     dk.s_in = state_grad; dk.s_in_transposed = true;
     for (const LinearAttentionPass *pass : {&dq, &dv, &dk})
-        if (int e = launch_linear_attention(*pass, (cudaStream_t)stream)) return cuda_fail("linear_attention_backward launch", e);
+        if (int e = launch_linear_attention(*pass, workspace, workspace_bytes, (cudaStream_t)stream)) return cuda_fail("linear_attention_backward launch", e);
     return RWKV7_OK;
 }
 

@@ -236,7 +236,13 @@ struct LinearAttentionPass {
     int device, num_sms;
 };
 bool linear_attention_supported(int64_t N);
-int launch_linear_attention(const LinearAttentionPass &p, cudaStream_t stream);
+// What a pass prefers as workspace; it takes any, down to none.
+size_t linear_attention_workspace_bytes(const LinearAttentionPass &p);
+int launch_linear_attention(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+// The tensor-core kernel (linear_attention_chunks.cu) for the shapes that it covers.
+bool linear_attention_chunks_supported(const LinearAttentionPass &p);
+size_t linear_attention_chunks_workspace_bytes(const LinearAttentionPass &p);
+int launch_linear_attention_chunks(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 
 // The norms before and after a block with its gate and residual scale; rows of C channels, parameters [C].
 struct ResidualNormArgs {

@@ -126,7 +126,12 @@ int launch_scan(const LinearAttentionPass &p, cudaStream_t stream) {
 
 bool linear_attention_supported(int64_t N) { return N == 32 || N == 64 || N == 128; }
 
-int launch_linear_attention(const LinearAttentionPass &p, cudaStream_t stream) {
+size_t linear_attention_workspace_bytes(const LinearAttentionPass &p) {
+    return linear_attention_chunks_supported(p) ? linear_attention_chunks_workspace_bytes(p) : 0;
+}
+
+int launch_linear_attention(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    if (linear_attention_chunks_supported(p)) return launch_linear_attention_chunks(p, workspace, workspace_bytes, stream);
     return p.bf16 ? launch_scan<__nv_bfloat16>(p, stream) : launch_scan<float>(p, stream);
 }
 
