@@ -10,15 +10,16 @@
 //
 // Four products of a chunk: P = A B^T [128 x 128], Y2 = A S [128 x 64], the sum for S' = B^T (w C) [64 x 64] and, once P carries
 // its decays and its mask, Y1 = P C [128 x 64].  A walk over the chunks is bound by HBM (64 KB a chunk, 1.5 us of an SM's share) if
-// two CTAs an SM take at most 3 us for one: so the chunk's chain of waits is kept short, not its arithmetic.  P stays in TMEM: read as
-// fp32, written back as the bf16 operand of its own product.
+// two CTAs an SM take at most 3 us for one: so the chunk's chain of waits is kept short.  P stays in TMEM: read as fp32, written
+// back as the bf16 operand of its own product.  Two threads share a row, which halves what is done between two products; c has two
+// buffers, for which the last part of w C takes the place of a as soon as a has been read.
 //
 // Precision: y is rounded to bf16, and so is P (once); S stays in fp32 registers and enters Y2 as hi + lo (16 bits and a
 // sign), because its errors would add up; the sum for S' takes w C as hi + mid + lo, all 24 bits, because S is an fp32 output.
 //
-// Warps 0-3 own one row (TMEM lane) a thread, warp 4 issues the products, warp 5 the loads.  The state's rows are those of b, on lanes
-// 0-63 forwards and 64-127 reversed: of the two 64-row blocks of that product's A operand the other one is whatever tile
-// lies beside b, and its lanes are not read.  (So the two warps with the smaller share of the triangle P update S.)
+// Warps 0-7 own half a row (TMEM lane) a thread, warp 8 issues the products, warp 9 the loads.  The state's rows are those of b, on
+// lanes 0-63 forwards and 64-127 reversed: of the two 64-row blocks of that product's A operand the other one is whatever
+// tile lies beside b, and its lanes are not read.  (So the warps with the smaller share of the triangle P update S.)
 //
 // Entries of c that are not finite would reach tokens on the other side of the mask (0 x inf): a chunk that has some takes
 // them as zero and sets what they do reach, the column's later tokens and the state's column, to NaN.
@@ -41,21 +42,23 @@ namespace {
 using namespace sm100;
 
 constexpr int kN = 64, kL = linear_attention_plan::kChunk;
-constexpr int kRowThreads = 128, kThreads = 192;
+constexpr int kRowThreads = 256, kThreads = kRowThreads + 64;
 constexpr uint32_t kTile = kL * 128;           // [128 tokens][64] bf16, 128-byte swizzle
-// Shared memory: a, b, c (in this order, see above), w C in three parts, S in two, tables, barriers.
-constexpr uint32_t kA = 0, kB = kTile, kC = 2 * kTile, kW = 3 * kTile, kS = 6 * kTile, kSPart = kN * 128;
-constexpr uint32_t kDec = kS + 2 * kSPart;     // d^0 .. d^128
-constexpr uint32_t kCol = kDec + 528;          // d^31 .. d^0 forwards, d^0 .. d^31 reversed
-constexpr uint32_t kBars = kCol + 128;
-constexpr uint32_t kBad = kBars + 112;         // per column the first (reversed: last) token that is not finite
+// Shared memory: a (then the last part of w C), b, c twice (in this order, see above), two parts of w C, S in two, tables, barriers.
+constexpr uint32_t kA = 0, kB = kTile, kC = 2 * kTile, kW = 4 * kTile, kS = 6 * kTile, kSPart = kN * 128;
+constexpr uint32_t kCol = kS + 2 * kSPart;     // d^31 .. d^0 forwards, d^0 .. d^31 reversed
+constexpr uint32_t kDec = kCol + 128;          // d^0 .. d^128
+constexpr uint32_t kBars = kDec + 520;
+constexpr uint32_t kBad = kBars + 120;         // per column the first (reversed: last) token that is not finite
 constexpr uint32_t kSmem = kBad + 256;
 static_assert(kSmem <= 115712, "two CTAs on an SM");
-// TMEM columns: P fp32 at 0 (its bf16 form on the first 64 of them, Y1 on the last), Y2 and the state's sum.
-constexpr uint32_t kP = 0, kY1 = 64, kY2 = 128, kKV = 192;
+// TMEM columns: P as fp32 at 0; as bf16 its first half on columns 0-31, its second on 96-127, where the threads that read
+// those columns put it; Y1 between them; Y2 and the state's sum.
+constexpr uint32_t kP = 0, kY1 = 32, kY2 = 128, kKV = 192;
+__host__ __device__ constexpr uint32_t p_operand(int kstep) { return kP + (kstep < 4 ? 0 : 64) + kstep * 8; }
 
 struct Maps {
-    CUtensorMap a, b, c;
+    CUtensorMap a, b, c, y;
 };
 
 struct ChunkArgs {
@@ -71,7 +74,8 @@ struct ChunkArgs {
     int *status;
 };
 
-enum Bar { kFullA, kFullB, kFullC, kPDone, kKvDone, kYDone, kSReady, kWReady, kPReady, kYRead, kEnd, kBarCount };
+enum Bar { kFullA, kFullB, kFullC, kFullC1, kPDone, kADone, kYDone, kKvDone, kSReady, kPReady, kWReady, kYRead, kYStored, kEnd, kBarCount };
+static_assert(kBarCount * 8 + 8 <= 120, "room for the barriers");
 
 // 16-byte piece `q` of a 128-byte row.
 __device__ __forceinline__ uint32_t piece(int row, int q) { return (uint32_t)row * 128u + (uint32_t)((q ^ (row & 7)) << 4); }
@@ -86,14 +90,7 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
 __device__ __forceinline__ float2 unpack2(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 __device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf2(v.x, v.y); }
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __fadd2_rn(a, make_float2(-b.x, -b.y)); }
-__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool rows_any(bool x) {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t)x) : "memory");
-    return r != 0;
-}
-
+__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // ADDS: only what a segment adds to the state.
 template <bool REVERSED, bool ADDS>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -109,13 +106,15 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + kBars + kBarCount * 8);
     float *dec = reinterpret_cast<float *>(smem + kDec), *col = reinterpret_cast<float *>(smem + kCol);
     int *bad_from = reinterpret_cast<int *>(smem + kBad);
+    volatile int *bad_chunk = reinterpret_cast<volatile int *>(tmem_slot + 1);   // the last chunk with entries that are not finite
     constexpr uint32_t kColumns = ADDS ? 64 : 256;
     if (tid == 0) {
         for (int i = 0; i < kBarCount; ++i)
-            mbar_init(bar + i, i == kSReady ? kN : i == kWReady || i == kPReady || i == kYRead ? kRowThreads : 1);
+            mbar_init(bar + i, i == kSReady ? 2 * kN : i >= kPReady && i <= kYStored ? kRowThreads : 1);
+        *bad_chunk = -1;
         mbar_fence_init();
     }
-    if (warp == 4) tmem_alloc(tmem_slot, kColumns);
+    if (warp == 8) tmem_alloc(tmem_slot, kColumns);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -142,126 +141,144 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         if (ok) ok = mbar_wait(bar + b, parity);
     };
 
-    if (warp == 5) {
+    if (warp == 9) {
         // ---- loads: a tile is refilled when the last product that reads it is done
         if (elect_one()) {
-            auto load = [&](int it, const CUtensorMap *map, uint32_t tile, Bar full) {
+            auto load = [&](int it, const CUtensorMap *map, uint32_t tile, int full) {
                 mbar_expect_tx(bar + full, kTile);
                 tma_load_3d(smem + tile, map, h * kN, first_token(it), bi, bar + full);
             };
-            if (count > 0) {
-                if (!ADDS) load(0, &maps.a, kA, kFullA);
-                load(0, &maps.b, kB, kFullB);
-                load(0, &maps.c, kC, kFullC);
-            }
-            int it = 0;
-            for (; it + 1 < count; ++it) {
+            auto load_ab = [&](int it) {
+                if (it >= count) return;
+                if (!ADDS) load(it, &maps.a, kA, kFullA);
+                load(it, &maps.b, kB, kFullB);
+            };
+            auto load_c = [&](int it) {
+                if (it < count) load(it, &maps.c, kC + (it & 1) * kTile, kFullC + (it & 1));
+            };
+            auto prefetch_ab = [&](int it) {   // (their loads have to wait for this chunk's products, and then find them in L2)
+                if (it >= count) return;
+                if (!ADDS) tma_prefetch_3d(&maps.a, h * kN, first_token(it), bi);
+                tma_prefetch_3d(&maps.b, h * kN, first_token(it), bi);
+            };
+            load_ab(0);
+            load_c(0);
+            load_c(1);
+            prefetch_ab(1);
+            for (int it = 0; it < count; ++it) {
                 const uint32_t ph = it & 1;
-                if (!ADDS) {
-                    if (!(ok = mbar_wait(bar + kPDone, ph))) break;
-                    load(it + 1, &maps.a, kA, kFullA);
+                if (it + 1 < count) {
+                    if (!(ok = mbar_wait(bar + kKvDone, ph))) break;
+                    load_ab(it + 1);
+                    prefetch_ab(it + 2);
                 }
-                if (!(ok = mbar_wait(bar + kKvDone, ph))) break;
-                load(it + 1, &maps.b, kB, kFullB);
-                if (!ADDS && !(ok = mbar_wait(bar + kYDone, ph))) break;
-                load(it + 1, &maps.c, kC, kFullC);
+                if (!ADDS) {   // y lies where c was
+                    if (!(ok = mbar_wait(bar + kYStored, ph))) break;
+                    tma_store_3d(&maps.y, h * kN, first_token(it), bi, smem + kC + (it & 1) * kTile);
+                    bulk_commit_group();
+                    if (it + 2 < count) bulk_wait_group_read<0>();
+                }
+                load_c(it + 2);
             }
-            // (after a time-out what is in flight lands before the CTA leaves: each tile's last phase, or the one after)
+            bulk_wait_group<0>();
+            // (after a time-out what is in flight lands before the CTA leaves: both phases of every tile)
             if (!ok)
-                for (int tile = kFullA; tile <= kFullC; ++tile)
-                    for (int i = 0; i < 2; ++i) mbar_wait(bar + tile, (uint32_t)((it + i) & 1), 100000u);
+                for (int tile = kFullA; tile <= kFullC1; ++tile)
+                    for (uint32_t i = 0; i < 2; ++i) mbar_wait(bar + tile, i, 100000u);
         }
-    } else if (warp == 4) {
+    } else if (warp == 8) {
         // ---- products
         if (elect_one()) {
             constexpr uint32_t id_p = make_idesc(kFmtBF16, 128, 128, false, false), id_y = make_idesc(kFmtBF16, 128, 64, false, true),
                                id_kv = make_idesc(kFmtBF16, 128, 64, true, true);
+            // one of the three parts of w C
+            auto add = [&](uint32_t part, bool first) {
+#pragma unroll
+                for (int k = 0; k < kL / 16; ++k)
+                    umma_f16(t_kv, make_smem_desc(base + (REVERSED ? kA : kB) + k * 2048, kTile, 1024),
+                             make_smem_desc(base + part + k * 2048, kTile, 1024), id_kv, !first || k > 0);
+            };
             for (int it = 0; it < count; ++it) {
                 const uint32_t ph = it & 1;
                 if (!ADDS) {
-                    ok = mbar_wait(bar + kFullA, ph) && mbar_wait(bar + kFullB, ph) && mbar_wait(bar + kSReady, ph) &&
-                         (it == 0 || mbar_wait(bar + kYRead, ph ^ 1));
+                    ok = mbar_wait(bar + kFullA, ph) && mbar_wait(bar + kFullB, ph) && (it == 0 || mbar_wait(bar + kYRead, ph ^ 1));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
                         umma_f16(tmem + kP, make_smem_desc(base + kA + k * 32, 16, 1024), make_smem_desc(base + kB + k * 32, 16, 1024), id_p, k > 0);
+                    umma_commit(bar + kPDone);
+                    if (!(ok = mbar_wait(bar + kSReady, ph))) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int k = 0; k < 2 * (kN / 16); ++k)   // S hi, S lo
                         umma_f16(tmem + kY2, make_smem_desc(base + kA + (k & 3) * 32, 16, 1024),
                                  make_smem_desc(base + kS + (k >> 2) * kSPart + (k & 3) * 2048, kSPart, 1024), id_y, k > 0);
-                    umma_commit(bar + kPDone);
+                    umma_commit(bar + kADone);
+                    ok = mbar_wait(bar + kPReady, ph) && mbar_wait(bar + kFullC + (it & 1), (uint32_t)(it >> 1) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kL / 16; ++k)
+                        umma_f16_ts(tmem + kY1, tmem + p_operand(k), make_smem_desc(base + kC + (it & 1) * kTile + k * 2048, kTile, 1024), id_y, k > 0);
+                    umma_commit(bar + kYDone);
                 }
                 ok = mbar_wait(bar + kWReady, ph) && (!ADDS || mbar_wait(bar + kFullB, ph));
                 if (!ok) break;
                 tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < 3 * (kL / 16); ++k)
-                    umma_f16(t_kv, make_smem_desc(base + (REVERSED ? kA : kB) + (k & 7) * 2048, kTile, 1024),
-                             make_smem_desc(base + kW + (k >> 3) * kTile + (k & 7) * 2048, kTile, 1024), id_kv, k > 0);
+                add(kW, true);
+                add(kW + kTile, false);
+                add(kA, false);
                 umma_commit(bar + kKvDone);
-                if (!ADDS) {
-                    if (!(ok = mbar_wait(bar + kPReady, ph))) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < kL / 16; ++k)
-                        umma_f16_ts(tmem + kY1, tmem + kP + k * 8, make_smem_desc(base + kC + k * 2048, kTile, 1024), id_y, k > 0);
-                    umma_commit(bar + kYDone);
-                }
             }
             umma_commit(bar + kEnd);
             ok = mbar_wait(bar + kEnd, 0) && ok;
         }
     } else {
         // ---- rows
-        const uint32_t t_lane = (uint32_t)(warp * 32) << 16;
-        const bool has_state = (warp >= 2) == REVERSED;   // uniform in a warp
-        const int bidx = tid & 63;
-        float2 S[kN / 2];
+        const int quarter = warp & 3, half = warp >> 2, row = tid & 127;
+        const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
+        const bool has_state = (quarter >= 2) == REVERSED;   // uniform in a warp
+        const int bidx = row & 63, c0 = half * (kN / 2);      // the thread's part of S: row bidx, 32 columns
+        float2 S[kN / 4];
 #pragma unroll
-        for (int j = 0; j < kN / 2; ++j) S[j] = make_float2(0.f, 0.f);
+        for (int j = 0; j < kN / 4; ++j) S[j] = make_float2(0.f, 0.f);
         if (tid <= kL) dec[tid] = power(tid);
-        if (tid == 0) dec[kL] = power(kL);
         if (tid < 32) col[tid] = power(REVERSED ? tid : 31 - tid);
+        constexpr int kNoToken = REVERSED ? -1 : kL;
+        if (tid < kN) bad_from[tid] = kNoToken;
+        float *parts = p.parts + (size_t)chain * p.segments * (kN * kN);
+        auto write = [&](float *dst) {
+#pragma unroll
+            for (int j = 0; j < kN / 4; ++j) {
+                dst[(c0 + 2 * j) * kN + bidx] = S[j].x;
+                dst[(c0 + 2 * j + 1) * kN + bidx] = S[j].y;
+            }
+        };
         if (has_state) {
             auto read = [&](const float *src, bool transposed) {
                 if (transposed) {
 #pragma unroll
-                    for (int j = 0; j < kN / 2; j += 2) {
-                        const float4 v = *reinterpret_cast<const float4 *>(src + bidx * kN + 2 * j);
+                    for (int j = 0; j < kN / 4; j += 2) {
+                        const float4 v = *reinterpret_cast<const float4 *>(src + bidx * kN + c0 + 2 * j);
                         S[j] = make_float2(v.x, v.y);
                         S[j + 1] = make_float2(v.z, v.w);
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < kN / 2; ++j) S[j] = make_float2(src[2 * j * kN + bidx], src[(2 * j + 1) * kN + bidx]);
+                    for (int j = 0; j < kN / 4; ++j) S[j] = make_float2(src[(c0 + 2 * j) * kN + bidx], src[(c0 + 2 * j + 1) * kN + bidx]);
                 }
             };
-            float *parts = p.parts + (size_t)chain * p.segments * (kN * kN);
             const float *s_in = p.s_in == nullptr ? nullptr : p.s_in + (size_t)chain * (kN * kN);
             if (ADDS) {
                 if (order == 0) {   // the state in front of everything: s_in may be overwritten before the last segment starts
                     if (s_in != nullptr) read(s_in, p.s_in_transposed);
+                    write(parts);
 #pragma unroll
-                    for (int j = 0; j < kN / 2; ++j) {
-                        parts[2 * j * kN + bidx] = S[j].x;
-                        parts[(2 * j + 1) * kN + bidx] = S[j].y;
-                        S[j] = make_float2(0.f, 0.f);
-                    }
+                    for (int j = 0; j < kN / 4; ++j) S[j] = make_float2(0.f, 0.f);
                 }
             } else if (p.segments > 1) {
-                read(parts, false);
-                for (int o = 1; o <= order; ++o) {
-                    const int s = REVERSED ? p.segments - o : o - 1;   // the segment whose sum this is
-                    const int64_t from = s * seg_tokens;
-                    const float f = power(max((int64_t)0, min((int64_t)len, from + seg_tokens) - from));
-                    const float *src = parts + (size_t)o * (kN * kN);
-#pragma unroll
-                    for (int j = 0; j < kN / 2; ++j) {
-                        S[j].x = fmaf(S[j].x, f, src[2 * j * kN + bidx]);
-                        S[j].y = fmaf(S[j].y, f, src[(2 * j + 1) * kN + bidx]);
-                    }
-                }
+                read(parts + (size_t)order * (kN * kN), false);
             } else if (s_in != nullptr) {
                 read(s_in, p.s_in_transposed);
             }
@@ -269,7 +286,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         // S as the operand of the next chunk's Y2: row b, columns c, hi and lo
         auto publish = [&] {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < 4; ++q) {
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -277,8 +294,8 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                     hi[e] = pack2(s);
                     lo[e] = pack2(sub2(s, unpack2(hi[e])));
                 }
-                sts16(base + kS + piece(bidx, q), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                sts16(base + kS + kSPart + piece(bidx, q), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                sts16(base + kS + piece(bidx, half * 4 + q), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                sts16(base + kS + kSPart + piece(bidx, half * 4 + q), make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
             fence_proxy_async();
             mbar_arrive(bar + kSReady);
@@ -286,94 +303,82 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         if (!ADDS && has_state && count > 0) publish();
         rows_sync();   // (the tables)
 
-        const float nan = __uint_as_float(0x7fffffffu);
         for (int it = 0; it < count; ++it) {
-            const uint32_t ph = it & 1;
+            const uint32_t ph = it & 1, tile_c = kC + (it & 1) * kTile;
             const int t0 = first_token(it), n = min(kL, len - t0);   // tokens of the chunk: all but the sequence's last have 128
-            // w C.  (The product that read the previous one is done; so is the one that read c.)
-            if (it > 0) wait(kKvDone, ph ^ 1);
-            wait(kFullC, ph);
-            if (n < kL) wait(kFullB, ph);
-            float2 finite = make_float2(0.f, 0.f);   // NaN if an entry is not
-            if (tid < n) {
-                const float w = dec[REVERSED ? tid + 1 : n - 1 - tid];
+            uint32_t own[4];   // where this thread's half row lies in a tile
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const uint4 u = lds16(base + kC + piece(tid, q));
-                    const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-                    uint32_t hi[4], mid[4], lo[4];
+            for (int q = 0; q < 4; ++q) own[q] = piece(row, half * 4 + q);
+
+            // c as the products may see it
+            wait((Bar)(kFullC + (it & 1)), (uint32_t)(it >> 1) & 1u);
+            if (n < kL) {   // (uniform) behind the sequence anything may stand
+                wait(kFullB, ph);
+                if (row >= n) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v = unpack2(in[e]);
-                        finite = __ffma2_rn(v, make_float2(0.f, 0.f), finite);
-                        float2 x = __fmul2_rn(v, make_float2(w, w));
-                        hi[e] = pack2(x);
-                        x = sub2(x, unpack2(hi[e]));
-                        mid[e] = pack2(x);
-                        lo[e] = pack2(sub2(x, unpack2(mid[e])));
+                    for (int q = 0; q < 4; ++q) {
+                        sts16(base + kB + own[q], make_uint4(0u, 0u, 0u, 0u));
+                        sts16(base + tile_c + own[q], make_uint4(0u, 0u, 0u, 0u));
                     }
-                    sts16(base + kW + piece(tid, q), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                    sts16(base + kW + kTile + piece(tid, q), make_uint4(mid[0], mid[1], mid[2], mid[3]));
-                    sts16(base + kW + 2 * kTile + piece(tid, q), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                }
-            } else {   // behind the sequence: what stands there may be anything
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    for (uint32_t tile : {kB, kC, kW, kW + kTile, kW + 2 * kTile}) sts16(base + tile + piece(tid, q), make_uint4(0u, 0u, 0u, 0u));
+                    fence_proxy_async();
                 }
             }
-            const bool any_bad = rows_any(finite.x + finite.y != 0.f);
-            if (any_bad) {
-                constexpr int kNoToken = REVERSED ? -1 : kL;
-                if (tid < kN) bad_from[tid] = kNoToken;
-                rows_sync();
-                if (tid < n) {
-                    for (int j = 0; j < kN; ++j) {
-                        const uint32_t at = piece(tid, j >> 3) + (j & 7) * 2;
-                        unsigned short *c = reinterpret_cast<unsigned short *>(smem + kC + at);
+            {
+                uint4 in[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) in[q] = lds16(base + tile_c + own[q]);
+                uint32_t all = 0;   // sign bits: an exponent of ones in the low or the high half of a word
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    for (uint32_t u : {in[q].x, in[q].y, in[q].z, in[q].w}) all |= ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                if (all != 0u) {
+                    for (int j = c0; j < c0 + kN / 2; ++j) {
+                        unsigned short *c = reinterpret_cast<unsigned short *>(smem + tile_c + piece(row, j >> 3) + (j & 7) * 2);
                         if ((*c & 0x7f80) != 0x7f80) continue;
                         *c = 0;
-                        for (int part = 0; part < 3; ++part) *reinterpret_cast<unsigned short *>(smem + kW + part * kTile + at) = 0;
-                        if (REVERSED) atomicMax(bad_from + j, tid);
-                        else atomicMin(bad_from + j, tid);
+                        if (REVERSED) atomicMax(bad_from + j, row);
+                        else atomicMin(bad_from + j, row);
                     }
+                    *bad_chunk = it;
+                    fence_proxy_async();
                 }
-                rows_sync();
             }
-            fence_proxy_async();
-            mbar_arrive(bar + kWReady);
 
             if (!ADDS) {
-                // P: decays and mask, and bf16
+                // P: decays and mask, and bf16.  Each warp takes two blocks of 32 columns, the outer one first (see p_operand).
                 wait(kPDone, ph);
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int i = 0; i < 2; ++i) {
+                    const int c = half == 0 ? i : 3 - i;
                     uint32_t out[16];
-                    if (REVERSED ? c < warp : c > warp) {
+                    if (REVERSED ? c < quarter : c > quarter) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) out[e] = 0u;
                     } else {
                         uint32_t v[32];
                         tmem_ld32(tmem + kP + t_lane + c * 32, v);
                         tmem_ld_wait();
-                        if (c == warp) {
+                        if (c == quarter) {
+                            const float *gap0 = dec + (REVERSED ? -lane : lane);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
-                                const int gap = REVERSED ? e - lane : lane - e;
-                                v[e] = gap >= 0 ? __float_as_uint(__uint_as_float(v[e]) * dec[max(gap, 0)]) : 0u;
+                                const bool seen = REVERSED ? e >= lane : e <= lane;
+                                const float g = seen ? gap0[REVERSED ? e : -e] : 0.f;
+                                v[e] = seen ? __float_as_uint(__uint_as_float(v[e]) * g) : 0u;
                             }
 #pragma unroll
                             for (int e = 0; e < 16; ++e) out[e] = pack_bf2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
                         } else {
                             // d^gap as a factor of the row and one of the column, neither with a negative power
-                            const float f = dec[REVERSED ? 32 * c - tid : tid - 32 * c - 31];
+                            const float f = dec[REVERSED ? 32 * c - row : row - 32 * c - 31];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const float2 g = *reinterpret_cast<const float2 *>(col + 2 * e);
-                                const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])),
-                                                            __fmul2_rn(g, make_float2(f, f)));
-                                out[e] = pack2(x);
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 g = *reinterpret_cast<const float4 *>(col + e);
+                                out[e / 2] = pack2(__fmul2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])),
+                                                              __fmul2_rn(make_float2(g.x, g.y), make_float2(f, f))));
+                                out[e / 2 + 1] = pack2(__fmul2_rn(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])),
+                                                                  __fmul2_rn(make_float2(g.z, g.w), make_float2(f, f))));
                             }
                         }
                         if (REVERSED && 32 * c + 32 > n) {   // (forwards no row of the sequence sees what is behind it)
@@ -384,81 +389,111 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                             }
                         }
                     }
-                    tmem_st16(tmem + kP + t_lane + c * 16, out);
+                    tmem_st16(tmem + p_operand(2 * c) + t_lane, out);
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(bar + kPReady);
             }
+
+            // w C in three parts.  (The product that read the previous ones is done, and a has been read.)
+            if (it > 0) wait(kKvDone, ph ^ 1);
+            if (!ADDS) wait(kADone, ph);
+            {
+                const float w = row < n ? dec[REVERSED ? row + 1 : n - 1 - row] : 0.f;
+                uint4 in[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) in[q] = lds16(base + tile_c + own[q]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t u[4] = {in[q].x, in[q].y, in[q].z, in[q].w};
+                    uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float2 x = __fmul2_rn(unpack2(u[e]), make_float2(w, w));
+                        hi[e] = pack2(x);
+                        x = sub2(x, unpack2(hi[e]));
+                        mid[e] = pack2(x);
+                        lo[e] = pack2(sub2(x, unpack2(mid[e])));
+                    }
+                    sts16(base + kW + own[q], make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                    sts16(base + kW + kTile + own[q], make_uint4(mid[0], mid[1], mid[2], mid[3]));
+                    sts16(base + kA + own[q], make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                }
+            }
+            fence_proxy_async();
+            mbar_arrive(bar + kWReady);
+
+            bool any_bad = false;   // (the same for all: every thread has looked at c before the products that are waited for)
+            if (!ADDS) {
+                // y, to where this thread's c was
+                wait(kYDone, ph);
+                tc_fence_after();
+                any_bad = *bad_chunk == it;
+                const float f = dec[REVERSED ? max(n - 1 - row, 0) : row + 1];
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t v[16], u[16];
+                    tmem_ld16(tmem + kY1 + t_lane + c0 + part * 16, v);
+                    tmem_ld16(tmem + kY2 + t_lane + c0 + part * 16, u);
+                    tmem_ld_wait();
+                    if (part == 1) {
+                        tc_fence_before();
+                        mbar_arrive(bar + kYRead);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), make_float2(f, f),
+                                                    make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                        u[e / 2] = pack2(x);
+                    }
+                    if (any_bad) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int from = bad_from[c0 + part * 16 + e];
+                            if (REVERSED ? row <= from : row >= from) u[e / 2] |= e & 1 ? 0x7fff0000u : 0x7fffu;
+                        }
+                    }
+                    if (row >= n) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) u[e] = 0u;
+                    }
+                    sts16(base + tile_c + own[2 * part], make_uint4(u[0], u[1], u[2], u[3]));
+                    sts16(base + tile_c + own[2 * part + 1], make_uint4(u[4], u[5], u[6], u[7]));
+                }
+                fence_proxy_async();
+                mbar_arrive(bar + kYStored);
+            }
             if (has_state) {
                 wait(kKvDone, ph);
                 tc_fence_after();
+                any_bad = *bad_chunk == it;
                 const float dn = dec[n];
+                uint32_t v[32];
+                tmem_ld32(t_kv + t_lane + c0, v);
+                tmem_ld_wait();
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t v[32];
-                    tmem_ld32(t_kv + t_lane + half * 32, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        S[half * 16 + e] = __ffma2_rn(S[half * 16 + e], make_float2(dn, dn),
-                                                      make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])));
-                }
+                for (int j = 0; j < kN / 4; ++j)
+                    S[j] = __ffma2_rn(S[j], make_float2(dn, dn), make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])));
                 if (any_bad) {
 #pragma unroll
-                    for (int j = 0; j < kN / 2; ++j) {
-                        if ((unsigned)bad_from[2 * j] < (unsigned)kL) S[j].x = nan;
-                        if ((unsigned)bad_from[2 * j + 1] < (unsigned)kL) S[j].y = nan;
+                    for (int j = 0; j < kN / 4; ++j) {
+                        if ((unsigned)bad_from[c0 + 2 * j] < (unsigned)kL) S[j].x = __uint_as_float(0x7fffffffu);
+                        if ((unsigned)bad_from[c0 + 2 * j + 1] < (unsigned)kL) S[j].y = __uint_as_float(0x7fffffffu);
                     }
                 }
                 tc_fence_before();
                 if (!ADDS && it + 1 < count) publish();
             }
             if (ADDS) {
-                if (any_bad) rows_sync();   // (bad_from has been read)
-                continue;
+                wait(kKvDone, ph);
+                any_bad = *bad_chunk == it;
             }
-            // y
-            wait(kYDone, ph);
-            tc_fence_after();
-            const float f = dec[REVERSED ? max(n - 1 - tid, 0) : tid + 1];
-            __nv_bfloat16 *y = p.y + (((int64_t)bi * p.T + t0 + tid) * p.H + h) * kN;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t v[32], u[32];
-                tmem_ld32(tmem + kY1 + t_lane + half * 32, v);
-                tmem_ld32(tmem + kY2 + t_lane + half * 32, u);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), make_float2(f, f),
-                                                make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                    v[e] = __float_as_uint(x.x);
-                    v[e + 1] = __float_as_uint(x.y);
-                }
-                if (any_bad) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int from = bad_from[half * 32 + e];
-                        if (REVERSED ? tid <= from : tid >= from) v[e] = __float_as_uint(nan);
-                    }
-                }
-                if (t0 + tid < p.T) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-                        if (tid < n) {
-                            uint32_t *w = &o.x;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = pack_bf2(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
-                        }
-                        *reinterpret_cast<uint4 *>(y + half * 32 + q * 8) = o;
-                    }
-                }
+            if (any_bad) {
+                rows_sync();   // (all have read it)
+                if (tid < kN) bad_from[tid] = kNoToken;
+                rows_sync();
             }
-            tc_fence_before();
-            mbar_arrive(bar + kYRead);
-            if (any_bad) rows_sync();
         }
         if (ok && !ADDS) {   // chunks behind the sequence
             const int from = begin + count * kL;
@@ -466,22 +501,45 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 *reinterpret_cast<uint4 *>(p.y + (((int64_t)bi * p.T + from + i / 8) * p.H + h) * kN + i % 8 * 8) = make_uint4(0u, 0u, 0u, 0u);
         }
         if (ok && has_state) {
-            float *dst = ADDS ? p.parts + ((size_t)chain * p.segments + order + 1) * (kN * kN)
-                              : order == p.segments - 1 && p.s_out != nullptr ? p.s_out + (size_t)chain * (kN * kN) : nullptr;
-            if (dst != nullptr) {
-#pragma unroll
-                for (int j = 0; j < kN / 2; ++j) {
-                    dst[2 * j * kN + bidx] = S[j].x;
-                    dst[(2 * j + 1) * kN + bidx] = S[j].y;
-                }
-            }
+            if (ADDS) write(parts + (size_t)(order + 1) * (kN * kN));
+            else if (order == p.segments - 1 && p.s_out != nullptr) write(p.s_out + (size_t)chain * (kN * kN));
         }
     }
     __syncwarp();
     if (!ok) atomicExch(p.status, (int)kDevTimeout);
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) tmem_dealloc(tmem, kColumns);
+    if (warp == 8) tmem_dealloc(tmem, kColumns);
+}
+
+// What each segment adds -> the state in front of each segment, in place: s_o = d^(tokens of o-1) s_(o-1) + part_o.  Four elements a
+// thread; the parts of several segments are on their way at once.
+__global__ void __launch_bounds__(256) segment_states_kernel(const ChunkArgs p, bool reversed) {
+    wait_for_previous();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int chain = (int)(i / (kN * kN / 4));
+    if (chain >= p.chains) return;
+    float4 *at = reinterpret_cast<float4 *>(p.parts) + (int64_t)chain * p.segments * (kN * kN / 4) + i % (kN * kN / 4);
+    const int len = p.lens == nullptr ? p.T : min(max(p.lens[chain / p.H], 0), p.T);
+    const float lambda = p.log_decay[chain % p.H];
+    const int64_t seg_tokens = (int64_t)p.chunks * kL;
+    float4 s = *at;
+    constexpr int kAhead = 8;
+    for (int o = 1; o < p.segments; o += kAhead) {
+        float4 part[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (o + j < p.segments) part[j] = at[(int64_t)(o + j) * (kN * kN / 4)];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (o + j >= p.segments) break;
+            const int64_t from = (reversed ? p.segments - (o + j) : o + j - 1) * seg_tokens;   // of the segment before this one
+            const int64_t tokens = max((int64_t)0, min((int64_t)len, from + seg_tokens) - from);
+            const float f = tokens == 0 ? 1.f : expf(lambda * (float)tokens);
+            s = make_float4(fmaf(s.x, f, part[j].x), fmaf(s.y, f, part[j].y), fmaf(s.z, f, part[j].z), fmaf(s.w, f, part[j].w));
+            at[(int64_t)(o + j) * (kN * kN / 4)] = s;
+        }
+    }
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -538,7 +596,7 @@ int launch_linear_attention_chunks(const LinearAttentionPass &p, void *workspace
     const int64_t chains = p.B * p.H;
     const Cut c = cut(chains, (p.T + kL - 1) / kL, p.num_sms, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, kN));
     Maps maps;
-    if (!describe(&maps.a, p.a, p) || !describe(&maps.b, p.b, p) || !describe(&maps.c, p.c, p)) return (int)cudaErrorInvalidValue;
+    if (!describe(&maps.a, p.a, p) || !describe(&maps.b, p.b, p) || !describe(&maps.c, p.c, p) || !describe(&maps.y, p.y, p)) return (int)cudaErrorInvalidValue;
     ChunkArgs args{};
     args.y = static_cast<__nv_bfloat16 *>(p.y);
     args.log_decay = p.log_decay;
@@ -557,6 +615,8 @@ int launch_linear_attention_chunks(const LinearAttentionPass &p, void *workspace
         const int64_t ctas = chains * (c.segments - 1);
         const cudaError_t e = p.reversed ? launch<true, true>(maps, args, ctas, p.device, stream) : launch<false, true>(maps, args, ctas, p.device, stream);
         if (e != cudaSuccess) return (int)e;
+        const cudaError_t f = launch_serialized(segment_states_kernel, (unsigned)((chains * (kN * kN / 4) + 255) / 256), 256u, 0, stream, args, p.reversed);
+        if (f != cudaSuccess) return (int)f;
     }
     const int64_t ctas = chains * c.segments;
     return (int)(p.reversed ? launch<true, false>(maps, args, ctas, p.device, stream) : launch<false, false>(maps, args, ctas, p.device, stream));
