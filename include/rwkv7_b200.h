@@ -606,7 +606,8 @@ int rwkv7_fused_residual_norm_backward(const rwkv7_tensor *residual, const rwkv7
  * logits [B,I,V] F32 or BF16, scores [B,I] F32.  A NaN among them counts as -inf, +inf as the largest finite number; a beam without
  * any logit above -inf has candidates of -inf only, which are chosen, by their index, when nothing else is left.  finished ([B,I]
  * I32, may be NULL): a beam whose entry is not zero has the candidate pad_token at its own score, and -inf for the rest.
- * workspace: rwkv7_beam_select_workspace_bytes, on 16 bytes.
+ * workspace: rwkv7_beam_select_workspace_bytes, on 16 bytes; the size depends on the SM count of the calling thread's current device.
+ * With less, down to 8 + 8 K bytes a beam (each of its three arrays rounded up to 16 bytes), fewer CTAs share a row; the choice is the same.
  */
 size_t rwkv7_beam_select_workspace_bytes(int64_t B, int64_t I, int64_t V, int64_t K);
 int rwkv7_beam_select(const rwkv7_tensor *logits, const rwkv7_tensor *scores, const rwkv7_tensor *finished, int64_t pad_token,

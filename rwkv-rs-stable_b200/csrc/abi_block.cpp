@@ -2,6 +2,7 @@
 // decay per head, the norms before and after a block, beam search.  Checks in the order and with the messages of abi.cpp.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -345,7 +346,13 @@ int rwkv7_fused_residual_norm_backward(const rwkv7_tensor *x_t, const rwkv7_tens
 // ---- beam search ------------------------------------------------------------------------------------------------------------
 
 size_t rwkv7_beam_select_workspace_bytes(int64_t B, int64_t I, int64_t V, int64_t K) {
-    return B <= 0 || I <= 0 || V <= 0 || K <= 0 ? 0 : beam_select_workspace_bytes(B, I, K);
+    if (B <= 0 || I <= 0 || V <= 0 || K <= 0 || I > 32 || K > 32) return 0;
+    BeamSelectArgs p{};
+    p.B = B; p.V = V; p.I = (int)I; p.K = (int)K;
+    p.num_sms = current_sms();
+    const size_t f32 = beam_select_workspace_bytes(p);
+    p.bf16 = true;
+    return std::max(f32, beam_select_workspace_bytes(p));
 }
 
 int rwkv7_beam_select(const rwkv7_tensor *logits_t, const rwkv7_tensor *scores_t, const rwkv7_tensor *finished_t, int64_t pad_token,
@@ -372,7 +379,7 @@ int rwkv7_beam_select(const rwkv7_tensor *logits_t, const rwkv7_tensor *scores_t
     RWKV7_TRY(check_of(logits, next, {B, K}, RWKV7_F32));
     RWKV7_TRY(check_of(logits, parents, {B, K}, RWKV7_I32));
     RWKV7_TRY(check_of(logits, tokens, {B, K}, RWKV7_I32));
-    if (K < 1 || K > 32 || I > 32 || V > INT32_MAX || K > I * V || B > INT32_MAX / I)
+    if (K < 1 || K > 32 || I > 32 || V > INT32_MAX || K > I * V || B > INT32_MAX / 32 / I)
         return fail(RWKV7_ERR_UNSUPPORTED, "Unsupported: beam_select of %lld out of %lld beams of %lld tokens, %lld searches (1 to 32 of at most 32)",
                     (long long)K, (long long)I, (long long)V, (long long)B);
     const TensorInfo outs[3] = {next, parents, tokens};
@@ -381,7 +388,6 @@ int rwkv7_beam_select(const rwkv7_tensor *logits_t, const rwkv7_tensor *scores_t
         for (int j = 0; j < i; ++j) RWKV7_TRY(check_apart(outs[i], outs[j]));
     }
     if (B == 0) return RWKV7_OK;
-    RWKV7_TRY(check_workspace("beam_select", workspace, workspace_bytes, beam_select_workspace_bytes(B, I, K)));
     BeamSelectArgs p{};
     p.logits = logits_t->data;
     p.scores = static_cast<const float *>(scores_t->data);
@@ -391,10 +397,11 @@ int rwkv7_beam_select(const rwkv7_tensor *logits_t, const rwkv7_tensor *scores_t
     p.tokens = static_cast<int *>(tokens_t->data);
     p.B = B; p.V = V; p.pad_token = pad_token; p.I = (int)I; p.K = (int)K;
     p.bf16 = logits_t->dtype == RWKV7_BF16;
+    RWKV7_TRY(check_workspace("beam_select", workspace, workspace_bytes, beam_select_min_workspace_bytes(p)));
     DeviceGuard guard(logits_t->device);
     if (guard.error() != cudaSuccess) return cuda_fail("cudaSetDevice", (int)guard.error());
     RWKV7_TRY(num_sms(logits_t->device, &p.num_sms));
-    if (int e = launch_beam_select(p, workspace, (cudaStream_t)stream)) return cuda_fail("beam_select launch", e);
+    if (int e = launch_beam_select(p, workspace, workspace_bytes, (cudaStream_t)stream)) return cuda_fail("beam_select launch", e);
     return RWKV7_OK;
 }
 

@@ -278,8 +278,9 @@ struct BeamSelectArgs {
     bool bf16;
     int num_sms;
 };
-size_t beam_select_workspace_bytes(int64_t B, int64_t I, int64_t K);
-int launch_beam_select(const BeamSelectArgs &p, void *workspace, cudaStream_t stream);
+size_t beam_select_workspace_bytes(const BeamSelectArgs &p);
+size_t beam_select_min_workspace_bytes(const BeamSelectArgs &p);
+int launch_beam_select(const BeamSelectArgs &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 constexpr int kMaxReordered = 48;   // tensors per launch
 struct BeamReorderArgs {
     struct Item {

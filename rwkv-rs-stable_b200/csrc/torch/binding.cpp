@@ -738,7 +738,10 @@ PyObject *beam_select(PyObject *const *a) {
     for (int i = 0; i < 3; ++i) od[i].set(out[i]);
     Workspace ws;
     if (a[5] != Py_None) ws.given(a[5]);
-    else if (logits.dim() == 3) ws.allocate(abi.rwkv7_beam_select_workspace_bytes(B, logits.size(1), logits.size(2), K), logits);
+    else if (logits.dim() == 3) {
+        const c10::cuda::OptionalCUDAGuard guard(logits.is_cuda() ? std::make_optional(logits.device()) : std::nullopt);
+        ws.allocate(abi.rwkv7_beam_select_workspace_bytes(B, logits.size(1), logits.size(2), K), logits);
+    }
     const rwkv7_stream st = stream_of(logits);
     call([&] { return abi.rwkv7_beam_select(ld.p, sd.p, fd.p, pad, od[0].p, od[1].p, od[2].p, ws.ptr, ws.bytes, st); });
     return tuple_of(out, 3);

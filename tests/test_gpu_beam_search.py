@@ -193,3 +193,22 @@ def test_reorder_captured(pkg, cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b[parents[0].long()]) for a, b in zip(out, states))
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "late", "plateau"])
+def test_rows_in_an_order(pkg, cuda, order):
+    """Many rows, so that a CTA goes over all of one: every logit larger than those before it; the best at the end; few above -inf in
+    front of many; a flood of equal ones."""
+    B, I, V = 200, 4, 40000
+    x = torch.arange(V, dtype=F32) / 64
+    if order == "falling":
+        x = x.flip(0)
+    elif order == "late":
+        x = torch.cat([torch.full((8180,), float("-inf")), torch.tensor([9.0, 3.0, 11.0]), torch.full((V - 8183 - 9000,), float("-inf")), x[:9000] / 16])
+    elif order == "plateau":
+        x = torch.where(x > 300, torch.full_like(x, 300.0), x)
+    assert x.numel() == V
+    logits = x.expand(B, I, V).contiguous().to(cuda)
+    scores = -torch.arange(I, dtype=F32).expand(B, I).contiguous().to(cuda) / 7
+    for K in (1, 4, 32):
+        _check(pkg, logits, scores, K)
