@@ -253,7 +253,7 @@ struct ResidualNormArgs {
     int64_t rows, C;
     bool layer;   // else rms
     bool bf16;
-    int num_sms;
+    int device, num_sms;
 };
 struct ResidualNormBackwardArgs {
     ResidualNormArgs f;                                    // (its outputs are not used)

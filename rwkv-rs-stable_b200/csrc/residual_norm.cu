@@ -4,10 +4,14 @@
 //   norm(v) = (v - mean v) / sqrt(var v + eps) gamma + beta        (layer; rms: without the mean)
 //
 // and its gradients.  Both are bound by the bytes of the rows: a CTA keeps a row in registers, eight channels a thread, so that every
-// element is read once and every result is rounded once, on its way out.  Means and variances are taken in turn (the variance from
-// the differences, which a large mean does not spoil), in fp32.
+// element is read once and every result is rounded once, on its way out.  It walks over rows with the parameters in registers
+// and the next row's loads on their way, for a row is a chain of sums over the block (forward four, backward six) and little else.
+// Means and variances are taken in turn (the variance from the differences, which a large mean does not spoil), in fp32.
+// Arithmetic goes two channels at a time, which halves the instructions that the backward pass would else be bound by.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "elements.cuh"
 #include "kernels.h"
@@ -16,237 +20,339 @@
 namespace rwkv7 {
 namespace {
 
-constexpr int kPer = 8;           // channels a thread
+constexpr int kPer = 8, kPairs = kPer / 2;   // channels a thread
 constexpr int kMaxWarps = 32;
-constexpr int kParams = 5;        // summed over the rows: scale, post gamma, post beta, pre gamma, pre beta
+constexpr int kParams = 5;                   // summed over the rows: scale, post gamma, post beta, pre gamma, pre beta
 
-// Eight channels of a row: neighbours where rows start on 16 bytes (VEC), else every threads-th.
-template <typename T, bool VEC>
-struct Lane {
-    int C, tid, threads;
-    __device__ int channel(int i) const { return VEC ? tid * kPer + i : tid + i * threads; }
-    __device__ bool any() const { return channel(0) < C; }
-    // (what lies outside the row counts as zero)
-    __device__ void load(float (&v)[kPer], const T *row) const {
-        if constexpr (VEC) {
-            if (any()) { ld8(v, row + tid * kPer); return; }
-        }
+struct Eight {
+    float2 v[kPairs];
+};
+__device__ __forceinline__ Eight all(float x) {
+    Eight r;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] = !VEC && channel(i) < C ? ldf(row + channel(i)) : 0.f;
+    for (int i = 0; i < kPairs; ++i) r.v[i] = make_float2(x, x);
+    return r;
+}
+__device__ __forceinline__ Eight operator*(const Eight &a, const Eight &b) {
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) r.v[i] = __fmul2_rn(a.v[i], b.v[i]);
+    return r;
+}
+__device__ __forceinline__ Eight operator+(const Eight &a, const Eight &b) {
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) r.v[i] = __fadd2_rn(a.v[i], b.v[i]);
+    return r;
+}
+__device__ __forceinline__ Eight fma(const Eight &a, const Eight &b, const Eight &c) {
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) r.v[i] = __ffma2_rn(a.v[i], b.v[i], c.v[i]);
+    return r;
+}
+__device__ __forceinline__ float total(const Eight &a) {
+    const float2 s = __fadd2_rn(__fadd2_rn(a.v[0], a.v[1]), __fadd2_rn(a.v[2], a.v[3]));
+    return s.x + s.y;
+}
+__device__ __forceinline__ float dot(const Eight &a, const Eight &b) {
+    float2 s = __fmul2_rn(a.v[0], b.v[0]);
+#pragma unroll
+    for (int i = 1; i < kPairs; ++i) s = __ffma2_rn(a.v[i], b.v[i], s);
+    return s.x + s.y;
+}
+
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw;
+template <>
+struct Raw<__nv_bfloat16> {
+    uint32_t r[kPairs];
+    __device__ Eight get() const {
+        Eight e;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) e.v[i] = make_float2(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u));
+        return e;
     }
-    __device__ void store(T *row, const float (&v)[kPer]) const {
+    __device__ void read(const __nv_bfloat16 *from) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(from);
+        r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
+    }
+    __device__ void set(int i, __nv_bfloat16 x) {
+        const uint32_t u = __bfloat16_as_ushort(x);
+        r[i / 2] = i & 1 ? (r[i / 2] & 0xffffu) | u << 16 : (r[i / 2] & 0xffff0000u) | u;
+    }
+};
+template <>
+struct Raw<float> {
+    float r[kPer];
+    __device__ Eight get() const {
+        Eight e;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) e.v[i] = make_float2(r[2 * i], r[2 * i + 1]);
+        return e;
+    }
+    __device__ void read(const float *from) {
+        const float4 a = *reinterpret_cast<const float4 *>(from), b = *reinterpret_cast<const float4 *>(from + 4);
+        r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
+        r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+    }
+    __device__ void set(int i, float x) { r[i] = x; }
+};
+
+// How much is known when a kernel is built: nothing (kOdd: rows that are not whole vectors, read by single elements); rows of whole
+// vectors (kVectors); these, no thread without channels, and every part of the operator there (kFull).  What the last leaves out are
+// some sixty branches a row.
+enum Form { kOdd, kVectors, kFull };
+
+// Eight channels of a row: neighbours, or, of odd rows, every threads-th.
+template <typename T, Form FORM>
+struct Lane {
+    static constexpr bool VEC = FORM != kOdd;
+    int C, tid, threads;
+    __device__ Lane(int64_t channels) : C((int)channels), tid((int)threadIdx.x), threads((int)blockDim.x) {}
+    __device__ int channel(int i) const { return VEC ? tid * kPer + i : tid + i * threads; }
+    __device__ bool inside(int i) const { return FORM == kFull || (VEC ? tid * kPer < C : channel(i) < C); }
+    // (what lies outside the row counts as zero)
+    __device__ Raw<T> load(const void *at, int64_t offset) const {
+        const T *row = static_cast<const T *>(at) + offset;
+        Raw<T> v{};
         if constexpr (VEC) {
-            if (any()) st8(row + tid * kPer, v);
+            if (inside(0)) {
+                v.read(row + tid * kPer);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-                if (channel(i) < C) stf(row + channel(i), v[i]);
+                if (inside(i)) v.set(i, row[channel(i)]);
+        }
+        return v;
+    }
+    __device__ void store(void *at, int64_t offset, const Eight &e) const {
+        T *row = static_cast<T *>(at) + offset;
+        const float v[kPer] = {e.v[0].x, e.v[0].y, e.v[1].x, e.v[1].y, e.v[2].x, e.v[2].y, e.v[3].x, e.v[3].y};
+        if constexpr (VEC) {
+            if (inside(0)) st8(row + tid * kPer, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (inside(i)) stf(row + channel(i), v[i]);
         }
     }
-    __device__ bool inside(int i) const { return VEC ? any() : channel(i) < C; }
+    // a - x; outside the row zero, or, where a thread is in it as a whole or not at all, anything: what it adds to a sum is taken out there
+    __device__ Eight minus(const Eight &a, float x) const {
+        Eight r;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            r.v[i] = __fadd2_rn(a.v[i], make_float2(-x, -x));
+            if constexpr (!VEC) r.v[i] = make_float2(inside(2 * i) ? r.v[i].x : 0.f, inside(2 * i + 1) ? r.v[i].y : 0.f);
+        }
+        return r;
+    }
+    __device__ float counted(float partial_sum) const { return !VEC || inside(0) ? partial_sum : 0.f; }
 };
 
-// The sums of `K` values over the block.  `slot` alternates between calls, so that one barrier a sum is enough.
-template <int K>
-__device__ __forceinline__ void block_sum(float (&v)[K], float (*shared)[kMaxWarps][2], int &slot, int warps) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// A parameter's eight channels: kept in registers where there is room for it, else read from L1 for every row.
+template <typename T, Form FORM, bool KEPT>
+struct Param {
+    const Lane<T, FORM> &lane;
+    const void *at;
+    Raw<T> kept;
+    __device__ Param(const Lane<T, FORM> &l, const void *p) : lane(l), at(p), kept{} {
+        if (KEPT && at != nullptr) kept = lane.load(at, 0);
+    }
+    __device__ Eight get() const {
+        if constexpr (KEPT) return kept.get();
+        else return at == nullptr ? all(0.f) : lane.load(at, 0).get();
+    }
+};
+
+// Sums over a block of at most MOST threads.  Two sets of slots in turn, so that one barrier a sum is enough.
+template <int MOST>
+struct Block {
+    float (*shared)[2][kMaxWarps];   // [set][value][warp], zero at first
+    int set = 0, warps = (int)blockDim.x >> 5;
+    __device__ __forceinline__ float of_warps(int k) const {
+        const float4 *part = reinterpret_cast<const float4 *>(shared[set][k]);
+        float4 s = part[0];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-    if (warps == 1) return;
-    if (lane == 0)
-#pragma unroll
-        for (int k = 0; k < K; ++k) shared[slot][warp][k] = v[k];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        float x = lane < warps ? shared[slot][lane][k] : 0.f;
+        for (int w = 1; w < MOST / 128; ++w) {
+            const float4 x = part[w];
+            s = make_float4(s.x + x.x, s.y + x.y, s.z + x.z, s.w + x.w);
+        }
+        return (s.x + s.y) + (s.z + s.w);
+    }
+    __device__ __forceinline__ float sum(float x) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        v[k] = x;
+        if (warps == 1) return x;
+        if ((threadIdx.x & 31) == 0) shared[set][0][threadIdx.x >> 5] = x;
+        __syncthreads();
+        x = of_warps(0);
+        set ^= 1;
+        return x;
     }
-    slot ^= 1;
+    // Two at once: the halves of the warp take one each after the first step.
+    __device__ __forceinline__ void sum2(float (&v)[2]) {
+        const int lane = threadIdx.x & 31;
+        const bool low = lane < 16;
+        float x = (low ? v[0] : v[1]) + __shfl_xor_sync(0xffffffffu, low ? v[1] : v[0], 16);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (warps == 1) {
+            v[0] = __shfl_sync(0xffffffffu, x, 0);
+            v[1] = __shfl_sync(0xffffffffu, x, 16);
+            return;
+        }
+        if ((lane & 15) == 0) shared[set][lane >> 4][threadIdx.x >> 5] = x;
+        __syncthreads();
+        v[0] = of_warps(0);
+        v[1] = of_warps(1);
+        set ^= 1;
+    }
+};
+__device__ __forceinline__ void clear(float (*shared)[2][kMaxWarps]) {
+    for (int i = threadIdx.x; i < 2 * 2 * kMaxWarps; i += blockDim.x) (&shared[0][0][0])[i] = 0.f;
+    __syncthreads();
 }
 
 // v -> (v - mean) / sqrt(var + eps); returns the reciprocal root.
-template <typename L>
-__device__ __forceinline__ float normalize(float (&v)[kPer], const L &lane, bool layer, float eps, float (*shared)[kMaxWarps][2], int &slot, int warps) {
-    float sum[1];
+template <typename L, typename B>
+__device__ __forceinline__ float normalize(Eight &v, const L &lane, bool layer, float eps, B &block) {
     const float inv = 1.f / (float)lane.C;
-    if (layer) {
-        sum[0] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) sum[0] += v[i];
-        block_sum(sum, shared, slot, warps);
-        const float mean = sum[0] * inv;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] = lane.inside(i) ? v[i] - mean : 0.f;
-    }
-    sum[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
-    block_sum(sum, shared, slot, warps);
-    const float r = 1.f / sqrtf(fmaf(sum[0], inv, eps));
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] *= r;
+    if (layer) v = lane.minus(v, block.sum(lane.counted(total(v))) * inv);
+    const float r = rsqrtf(fmaf(block.sum(lane.counted(dot(v, v))), inv, eps));
+    v = v * all(r);
     return r;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(1024)
+template <typename T, Form FORM, int MOST, int RESIDENT>
+__global__ void __launch_bounds__(MOST, RESIDENT)
 residual_norm_kernel(const ResidualNormArgs p) {
-    __shared__ float shared[2][kMaxWarps][2];
-    const Lane<T, VEC> lane{(int)p.C, (int)threadIdx.x, (int)blockDim.x};
-    const int warps = (int)blockDim.x >> 5;
-    int slot = 0;
+    __shared__ __align__(16) float shared[2][2][kMaxWarps];
+    const Lane<T, FORM> lane(p.C);
+    clear(shared);
+    Block<MOST> block{shared};
     wait_for_previous();
-    auto param = [&](float (&v)[kPer], const void *q, float absent) {
-        if (q != nullptr) lane.load(v, static_cast<const T *>(q));
-        else
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) v[i] = absent;
+    let_next_in();
+    constexpr bool kAll = FORM == kFull;
+    const bool has_block = kAll || p.block_output != nullptr, has_gate = kAll || p.gate != nullptr, post = kAll || p.post_gamma != nullptr,
+               has_scale = kAll || p.residual_scale != nullptr, pre = kAll || p.normed != nullptr;
+    Raw<T> x_in, h_in{}, g_in{};
+    auto load = [&](int64_t row) {
+        x_in = lane.load(p.residual, row * p.C);
+        if (has_block) h_in = lane.load(p.block_output, row * p.C);
+        if (has_gate) g_in = lane.load(p.gate, row * p.C);
     };
-    const int64_t at = (int64_t)blockIdx.x * p.C;
-    float x[kPer], u[kPer], w[kPer];
-    lane.load(x, static_cast<const T *>(p.residual) + at);
-    if (p.block_output != nullptr) {
-        lane.load(u, static_cast<const T *>(p.block_output) + at);
-        float g[kPer];
-        param(g, p.gate == nullptr ? nullptr : static_cast<const T *>(p.gate) + at, 1.f);
-        if (p.post_gamma != nullptr) {
-            normalize(u, lane, p.layer, p.epsilon, shared, slot, warps);
-            param(w, p.post_gamma, 1.f);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) u[i] *= w[i];
-            param(w, p.post_beta, 0.f);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) u[i] += w[i];
+    load(blockIdx.x);
+    const Param<T, FORM, sizeof(T) == 2> scale(lane, p.residual_scale), post_gamma(lane, p.post_gamma), post_beta(lane, p.post_beta), pre_gamma(lane, p.pre_gamma),
+        pre_beta(lane, p.pre_beta);
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const int64_t at = row * p.C;
+        Eight x = x_in.get(), u = h_in.get(), g = g_in.get();
+        if (row + gridDim.x < p.rows) load(row + gridDim.x);
+        if (has_block) {
+            if (post) {
+                normalize(u, lane, p.layer, p.epsilon, block);
+                u = fma(u, post_gamma.get(), post_beta.get());
+            }
+            if (has_gate) u = g * u;
+            x = has_scale ? fma(scale.get(), u, x) : x + u;
+            lane.store(p.next_residual, at, x);
         }
-        param(w, p.residual_scale, 1.f);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = lane.inside(i) ? fmaf(w[i], g[i] * u[i], x[i]) : 0.f;
-        lane.store(static_cast<T *>(p.next_residual) + at, x);
+        if (!pre) continue;
+        normalize(x, lane, p.layer, p.epsilon, block);
+        lane.store(p.normed, at, fma(x, pre_gamma.get(), pre_beta.get()));
     }
-    if (p.normed == nullptr) return;
-    normalize(x, lane, p.layer, p.epsilon, shared, slot, warps);
-    param(w, p.pre_gamma, 1.f);
-    param(u, p.pre_beta, 0.f);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = fmaf(x[i], w[i], u[i]);
-    lane.store(static_cast<T *>(p.normed) + at, x);
 }
 
 // (dy gamma) -> the gradient behind the normalisation: r (g - mean g - hat mean(g hat)), rms without the first mean.
-template <typename L>
-__device__ __forceinline__ void normalize_backward(float (&g)[kPer], const float (&hat)[kPer], float r, const L &lane, bool layer,
-                                                   float (*shared)[kMaxWarps][2], int &slot, int warps) {
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        sum[0] += g[i];
-        sum[1] = fmaf(g[i], hat[i], sum[1]);
-    }
-    block_sum(sum, shared, slot, warps);
+template <typename L, typename B>
+__device__ __forceinline__ Eight normalize_backward(const Eight &g, const Eight &hat, float r, const L &lane, bool layer, B &block) {
+    float sum[2] = {lane.counted(total(g)), lane.counted(dot(g, hat))};
+    block.sum2(sum);
     const float inv = 1.f / (float)lane.C;
-    const float mean = layer ? sum[0] * inv : 0.f, dot = sum[1] * inv;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) g[i] = lane.inside(i) ? r * (g[i] - mean - hat[i] * dot) : 0.f;
+    return fma(hat, all(-r * sum[1] * inv), lane.minus(g, layer ? sum[0] * inv : 0.f) * all(r));
 }
 
-// Rows in turn; a thread sums the gradients of its channels' parameters over its rows and leaves them to the second kernel.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(1024)
+// A thread sums the gradients of its channels' parameters over its rows, in registers, and leaves them to the second kernel.
+template <typename T, Form FORM, int MOST, int RESIDENT>
+__global__ void __launch_bounds__(MOST, RESIDENT)
 residual_norm_backward_kernel(const ResidualNormBackwardArgs p, float *partials) {
-    __shared__ float shared[2][kMaxWarps][2];
-    const Lane<T, VEC> lane{(int)p.f.C, (int)threadIdx.x, (int)blockDim.x};
-    const int warps = (int)blockDim.x >> 5;
-    int slot = 0;
+    __shared__ __align__(16) float shared[2][2][kMaxWarps];
+    const Lane<T, FORM> lane(p.f.C);
+    clear(shared);
+    Block<MOST> block{shared};
     wait_for_previous();
-    auto param = [&](float (&v)[kPer], const void *q, float absent) {
-        if (q != nullptr) lane.load(v, static_cast<const T *>(q));
-        else
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) v[i] = absent;
+    let_next_in();
+    constexpr bool kAll = FORM == kFull;
+    const bool has_block = kAll || p.f.block_output != nullptr, has_gate = kAll || p.f.gate != nullptr, post = kAll || p.f.post_gamma != nullptr,
+               has_scale = kAll || p.f.residual_scale != nullptr, pre = kAll || p.normed_grad != nullptr,
+               has_grad = kAll || p.next_residual_grad != nullptr;
+    Raw<T> x_in, h_in{}, g_in{}, dz_in{}, dx_in{};
+    auto load = [&](int64_t row) {
+        x_in = lane.load(p.f.residual, row * p.f.C);
+        if (has_block) h_in = lane.load(p.f.block_output, row * p.f.C);
+        if (has_gate) g_in = lane.load(p.f.gate, row * p.f.C);
+        if (pre) dz_in = lane.load(p.normed_grad, row * p.f.C);
+        if (has_grad) dx_in = lane.load(p.next_residual_grad, row * p.f.C);
     };
-    float sum[kParams][kPer] = {};
-    const bool block = p.f.block_output != nullptr, post = p.f.post_gamma != nullptr, pre = p.normed_grad != nullptr;
-    for (int64_t r = blockIdx.x; r < p.f.rows; r += gridDim.x) {
-        const int64_t at = r * p.f.C;
-        float x[kPer], h[kPer], g[kPer], u[kPer], w[kPer], dx[kPer];
-        lane.load(x, static_cast<const T *>(p.f.residual) + at);
+    constexpr bool kAhead = sizeof(T) == 2;   // (five fp32 rows on their way would not leave room for the one at hand)
+    if (kAhead) load(blockIdx.x);
+    const Param<T, FORM, false> scale_in(lane, p.f.residual_scale), post_gamma(lane, p.f.post_gamma), post_beta(lane, p.f.post_beta),
+        pre_gamma(lane, p.f.pre_gamma);
+    auto scale = [&] { return has_scale ? scale_in.get() : all(1.f); };
+    Eight sum[kParams];
+#pragma unroll
+    for (int k = 0; k < kParams; ++k) sum[k] = all(0.f);
+    for (int64_t row = blockIdx.x; row < p.f.rows; row += gridDim.x) {
+        const int64_t at = row * p.f.C;
+        if (!kAhead) load(row);
+        Eight x = x_in.get(), h = h_in.get();
+        const Eight g = has_gate ? g_in.get() : all(1.f);
+        Eight dz = dz_in.get(), dx = dx_in.get();   // (zero where there is none)
+        if (kAhead && row + gridDim.x < p.f.rows) load(row + gridDim.x);
+        Eight u = h;
         float rh = 0.f;
-        if (block) {
-            lane.load(h, static_cast<const T *>(p.f.block_output) + at);
-            param(g, p.f.gate == nullptr ? nullptr : static_cast<const T *>(p.f.gate) + at, 1.f);
+        if (has_block) {
             if (post) {
-                rh = normalize(h, lane, p.f.layer, p.f.epsilon, shared, slot, warps);
-                param(w, p.f.post_gamma, 1.f);
-                param(u, p.f.post_beta, 0.f);
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) u[i] = fmaf(h[i], w[i], u[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) u[i] = h[i];
+                rh = normalize(h, lane, p.f.layer, p.f.epsilon, block);
+                u = fma(h, post_gamma.get(), post_beta.get());
             }
-            param(w, p.f.residual_scale, 1.f);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) x[i] = lane.inside(i) ? fmaf(w[i], g[i] * u[i], x[i]) : 0.f;
+            x = fma(scale(), g * u, x);
         }
         if (pre) {
-            const float rx = normalize(x, lane, p.f.layer, p.f.epsilon, shared, slot, warps);
-            lane.load(dx, static_cast<const T *>(p.normed_grad) + at);
-            param(w, p.f.pre_gamma, 1.f);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                sum[3][i] = fmaf(dx[i], x[i], sum[3][i]);
-                sum[4][i] += dx[i];
-                dx[i] *= w[i];
-            }
-            normalize_backward(dx, x, rx, lane, p.f.layer, shared, slot, warps);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) dx[i] = 0.f;
+            const float rx = normalize(x, lane, p.f.layer, p.f.epsilon, block);
+            sum[3] = fma(dz, x, sum[3]);
+            sum[4] = sum[4] + dz;
+            dx = dx + normalize_backward(dz * pre_gamma.get(), x, rx, lane, p.f.layer, block);
         }
-        if (p.next_residual_grad != nullptr) {
-            lane.load(w, static_cast<const T *>(p.next_residual_grad) + at);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) dx[i] += w[i];
-        }
-        lane.store(static_cast<T *>(p.residual_grad) + at, dx);
-        if (!block) continue;
-        param(w, p.f.residual_scale, 1.f);
-        float dg[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            sum[0][i] = fmaf(dx[i], g[i] * u[i], sum[0][i]);
-            dg[i] = dx[i] * w[i] * u[i];
-            dx[i] = dx[i] * w[i] * g[i];   // the gradient of u from here on
-        }
-        if (p.gate_grad != nullptr) lane.store(static_cast<T *>(p.gate_grad) + at, dg);
+        lane.store(p.residual_grad, at, dx);
+        if (!has_block) continue;
+        sum[0] = fma(dx, g * u, sum[0]);
+        dx = dx * scale();
+        if (has_gate) lane.store(p.gate_grad, at, dx * u);
+        dx = dx * g;   // the gradient of u
         if (post) {
-            param(w, p.f.post_gamma, 1.f);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                sum[1][i] = fmaf(dx[i], h[i], sum[1][i]);
-                sum[2][i] += dx[i];
-                dx[i] *= w[i];
-            }
-            normalize_backward(dx, h, rh, lane, p.f.layer, shared, slot, warps);
+            sum[1] = fma(dx, h, sum[1]);
+            sum[2] = sum[2] + dx;
+            dx = normalize_backward(dx * post_gamma.get(), h, rh, lane, p.f.layer, block);
         }
-        lane.store(static_cast<T *>(p.block_output_grad) + at, dx);
+        lane.store(p.block_output_grad, at, dx);
     }
 #pragma unroll
     for (int k = 0; k < kParams; ++k) {
         if (p.param_grads[k] == nullptr) continue;
         float *row = partials + ((int64_t)k * gridDim.x + blockIdx.x) * p.f.C;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (lane.inside(i)) row[lane.channel(i)] = sum[k][i];
+        for (int i = 0; i < kPairs; ++i) {
+            if (lane.inside(2 * i)) row[lane.channel(2 * i)] = sum[k].v[i].x;
+            if (lane.inside(2 * i + 1)) row[lane.channel(2 * i + 1)] = sum[k].v[i].y;
+        }
     }
 }
 
-// Sums the CTAs' parts of the parameters' gradients: one warp for 32 channels of one parameter, in the order of the CTAs.
+// Sums the CTAs' parts of the parameters' gradients, 32 channels of one parameter a CTA: eight warps in turn, then in their order.
 template <typename T>
 __global__ void __launch_bounds__(256)
 residual_norm_params_kernel(const ResidualNormBackwardArgs p, const float *partials, int parts) {
@@ -258,8 +364,17 @@ residual_norm_params_kernel(const ResidualNormBackwardArgs p, const float *parti
     wait_for_previous();
     if (p.param_grads[k] == nullptr) return;
     float sum = 0.f;
-    if (c < p.f.C)
-        for (int i = warp; i < parts; i += 8) sum += partials[((int64_t)k * parts + i) * p.f.C + c];
+    if (c < p.f.C) {
+        const float *at = partials + (int64_t)k * parts * p.f.C + c;
+        constexpr int kAhead = 8;
+        for (int i = warp; i < parts; i += 8 * kAhead) {
+            float x[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) x[j] = i + 8 * j < parts ? at[(int64_t)(i + 8 * j) * p.f.C] : 0.f;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) sum += x[j];
+        }
+    }
     shared[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && c < p.f.C) {
@@ -271,15 +386,28 @@ residual_norm_params_kernel(const ResidualNormBackwardArgs p, const float *parti
 
 unsigned threads_for(int64_t C) { return (unsigned)(((C + kPer - 1) / kPer + 31) / 32 * 32); }
 
-int backward_parts(int64_t rows, int num_sms) {
-    const int64_t most = (int64_t)num_sms * 2;
-    return (int)(rows < most ? rows : most);
+// CTAs of the backward pass: what its registers let an SM hold of blocks of that size.
+int backward_parts(int64_t rows, int64_t C, int num_sms) {
+    const int64_t threads = threads_for(C), resident = std::max<int64_t>(1, 512 / threads);
+    return (int)std::min<int64_t>(rows, (int64_t)num_sms * resident);
 }
 
-template <typename T, bool VEC>
+template <typename T, Form FORM>
+int launch_forward(const ResidualNormArgs &p, cudaStream_t stream) {
+    const unsigned threads = threads_for(p.C);
+    const unsigned ctas = (unsigned)std::min<int64_t>(p.rows, (int64_t)p.num_sms * std::max(1u, 768 / threads));
+    const auto kernel = threads <= 256 ? residual_norm_kernel<T, FORM, 256, 3>
+                        : threads <= 512 ? residual_norm_kernel<T, FORM, 512, 1> : residual_norm_kernel<T, FORM, 1024, 1>;
+    return (int)launch_serialized(kernel, ctas, threads, 0, stream, p);
+}
+
+template <typename T, Form FORM>
 int launch_backward(const ResidualNormBackwardArgs &p, float *partials, cudaStream_t stream) {
-    const int parts = backward_parts(p.f.rows, p.f.num_sms);
-    cudaError_t e = launch_serialized(residual_norm_backward_kernel<T, VEC>, (unsigned)parts, threads_for(p.f.C), 0, stream, p, partials);
+    const int parts = backward_parts(p.f.rows, p.f.C, p.f.num_sms);
+    const unsigned threads = threads_for(p.f.C);
+    const auto kernel = threads <= 256 ? residual_norm_backward_kernel<T, FORM, 256, 2>
+                        : threads <= 512 ? residual_norm_backward_kernel<T, FORM, 512, 1> : residual_norm_backward_kernel<T, FORM, 1024, 1>;
+    const cudaError_t e = launch_serialized(kernel, (unsigned)parts, threads, 0, stream, p, partials);
     bool any = false;
     for (void *g : p.param_grads) any = any || g != nullptr;
     if (e != cudaSuccess || !any) return (int)e;
@@ -292,21 +420,24 @@ int launch_backward(const ResidualNormBackwardArgs &p, float *partials, cudaStre
 int64_t residual_norm_max_channels() { return 1024 * kPer; }
 
 size_t residual_norm_backward_workspace_bytes(int64_t rows, int64_t C, int num_sms) {
-    return (size_t)backward_parts(rows, num_sms) * (size_t)C * kParams * sizeof(float);
+    return (size_t)backward_parts(rows, C, num_sms) * (size_t)C * kParams * sizeof(float);
 }
 
 int launch_residual_norm(const ResidualNormArgs &p, cudaStream_t stream) {
-    const bool vec = p.C % kPer == 0;
-    const auto kernel = p.bf16 ? (vec ? residual_norm_kernel<__nv_bfloat16, true> : residual_norm_kernel<__nv_bfloat16, false>)
-                               : (vec ? residual_norm_kernel<float, true> : residual_norm_kernel<float, false>);
-    return (int)launch_serialized(kernel, (unsigned)p.rows, threads_for(p.C), 0, stream, p);
+    const bool full = p.C % (32 * kPer) == 0 && p.block_output != nullptr && p.gate != nullptr && p.residual_scale != nullptr && p.post_gamma != nullptr && p.normed != nullptr;
+    if (p.C % kPer != 0) return p.bf16 ? launch_forward<__nv_bfloat16, kOdd>(p, stream) : launch_forward<float, kOdd>(p, stream);
+    if (!full) return p.bf16 ? launch_forward<__nv_bfloat16, kVectors>(p, stream) : launch_forward<float, kVectors>(p, stream);
+    return p.bf16 ? launch_forward<__nv_bfloat16, kFull>(p, stream) : launch_forward<float, kFull>(p, stream);
 }
 
 int launch_residual_norm_backward(const ResidualNormBackwardArgs &p, void *workspace, cudaStream_t stream) {
     float *partials = static_cast<float *>(workspace);
-    const bool vec = p.f.C % kPer == 0;
-    if (p.f.bf16) return vec ? launch_backward<__nv_bfloat16, true>(p, partials, stream) : launch_backward<__nv_bfloat16, false>(p, partials, stream);
-    return vec ? launch_backward<float, true>(p, partials, stream) : launch_backward<float, false>(p, partials, stream);
+    const ResidualNormArgs &f = p.f;
+    const bool full = f.C % (32 * kPer) == 0 && f.block_output != nullptr && f.gate != nullptr && f.residual_scale != nullptr && f.post_gamma != nullptr &&
+                      p.normed_grad != nullptr && p.next_residual_grad != nullptr;
+    if (f.C % kPer != 0) return f.bf16 ? launch_backward<__nv_bfloat16, kOdd>(p, partials, stream) : launch_backward<float, kOdd>(p, partials, stream);
+    if (!full) return f.bf16 ? launch_backward<__nv_bfloat16, kVectors>(p, partials, stream) : launch_backward<float, kVectors>(p, partials, stream);
+    return f.bf16 ? launch_backward<__nv_bfloat16, kFull>(p, partials, stream) : launch_backward<float, kFull>(p, partials, stream);
 }
 
 }  // namespace rwkv7
