@@ -239,6 +239,8 @@ bool linear_attention_supported(int64_t N);
 // What a pass prefers as workspace; it takes any, down to none.
 size_t linear_attention_workspace_bytes(const LinearAttentionPass &p);
 int launch_linear_attention(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+// parts [chain][segment][N][N], what each segment but the last adds behind the state in front of all -> the state in front of each.
+int launch_segment_states(const LinearAttentionPass &p, float *parts, int64_t segments, int64_t tokens, cudaStream_t stream);
 // The tensor-core kernel (linear_attention_chunks.cu) for the shapes that it covers.
 bool linear_attention_chunks_supported(const LinearAttentionPass &p);
 size_t linear_attention_chunks_workspace_bytes(const LinearAttentionPass &p);

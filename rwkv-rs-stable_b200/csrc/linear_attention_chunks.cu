@@ -512,36 +512,6 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     if (warp == 8) tmem_dealloc(tmem, kColumns);
 }
 
-// What each segment adds -> the state in front of each segment, in place: s_o = d^(tokens of o-1) s_(o-1) + part_o.  Four elements a
-// thread; the parts of several segments are on their way at once.
-__global__ void __launch_bounds__(256) segment_states_kernel(const ChunkArgs p, bool reversed) {
-    wait_for_previous();
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int chain = (int)(i / (kN * kN / 4));
-    if (chain >= p.chains) return;
-    float4 *at = reinterpret_cast<float4 *>(p.parts) + (int64_t)chain * p.segments * (kN * kN / 4) + i % (kN * kN / 4);
-    const int len = p.lens == nullptr ? p.T : min(max(p.lens[chain / p.H], 0), p.T);
-    const float lambda = p.log_decay[chain % p.H];
-    const int64_t seg_tokens = (int64_t)p.chunks * kL;
-    float4 s = *at;
-    constexpr int kAhead = 8;
-    for (int o = 1; o < p.segments; o += kAhead) {
-        float4 part[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-            if (o + j < p.segments) part[j] = at[(int64_t)(o + j) * (kN * kN / 4)];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (o + j >= p.segments) break;
-            const int64_t from = (reversed ? p.segments - (o + j) : o + j - 1) * seg_tokens;   // of the segment before this one
-            const int64_t tokens = max((int64_t)0, min((int64_t)len, from + seg_tokens) - from);
-            const float f = tokens == 0 ? 1.f : expf(lambda * (float)tokens);
-            s = make_float4(fmaf(s.x, f, part[j].x), fmaf(s.y, f, part[j].y), fmaf(s.z, f, part[j].z), fmaf(s.w, f, part[j].w));
-            at[(int64_t)(o + j) * (kN * kN / 4)] = s;
-        }
-    }
-}
-
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -588,13 +558,13 @@ bool linear_attention_chunks_supported(const LinearAttentionPass &p) { return p.
 size_t linear_attention_chunks_workspace_bytes(const LinearAttentionPass &p) {
     using namespace linear_attention_plan;
     const int64_t chains = p.B * p.H;
-    return state_bytes(chains, cut(chains, (p.T + kL - 1) / kL, p.num_sms, INT64_MAX).segments, kN);
+    return state_bytes(chains, cut(chains, (p.T + kL - 1) / kL, (int64_t)p.num_sms * kResident, 1, INT64_MAX).segments, kN);
 }
 
 int launch_linear_attention_chunks(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
     using namespace linear_attention_plan;
     const int64_t chains = p.B * p.H;
-    const Cut c = cut(chains, (p.T + kL - 1) / kL, p.num_sms, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, kN));
+    const Cut c = cut(chains, (p.T + kL - 1) / kL, (int64_t)p.num_sms * kResident, 1, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, kN));
     Maps maps;
     if (!describe(&maps.a, p.a, p) || !describe(&maps.b, p.b, p) || !describe(&maps.c, p.c, p) || !describe(&maps.y, p.y, p)) return (int)cudaErrorInvalidValue;
     ChunkArgs args{};
@@ -615,8 +585,7 @@ int launch_linear_attention_chunks(const LinearAttentionPass &p, void *workspace
         const int64_t ctas = chains * (c.segments - 1);
         const cudaError_t e = p.reversed ? launch<true, true>(maps, args, ctas, p.device, stream) : launch<false, true>(maps, args, ctas, p.device, stream);
         if (e != cudaSuccess) return (int)e;
-        const cudaError_t f = launch_serialized(segment_states_kernel, (unsigned)((chains * (kN * kN / 4) + 255) / 256), 256u, 0, stream, args, p.reversed);
-        if (f != cudaSuccess) return (int)f;
+        if (int f = launch_segment_states(p, args.parts, c.segments, c.chunks * kL, stream)) return f;
     }
     const int64_t ctas = chains * c.segments;
     return (int)(p.reversed ? launch<true, false>(maps, args, ctas, p.device, stream) : launch<false, false>(maps, args, ctas, p.device, stream));
