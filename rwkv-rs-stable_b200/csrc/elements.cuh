@@ -40,12 +40,22 @@ __device__ __forceinline__ void st8(float *p, const float (&v)[8]) {
 __device__ __forceinline__ void st8(__nv_bfloat16 *p, const float (&v)[8]) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
 }
-// Four elements to shared memory as fp32; N neighbouring results.
+// Four elements to shared memory as fp32; N (2 or 4) neighbours.
 __device__ __forceinline__ void st4(float *to, const float *from) { *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(from); }
 __device__ __forceinline__ void st4(float *to, const __nv_bfloat16 *from) {
     const uint2 u = *reinterpret_cast<const uint2 *>(from);
     *reinterpret_cast<float4 *>(to) = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
                                                   __uint_as_float(u.y & 0xffff0000u));
+}
+template <int N>
+__device__ __forceinline__ void ldn(float (&v)[N], const float *p) {
+    if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const float2 x = *reinterpret_cast<const float2 *>(p);
+        v[0] = x.x; v[1] = x.y;
+    }
 }
 template <int N>
 __device__ __forceinline__ void stn(float *p, const float (&v)[N]) {

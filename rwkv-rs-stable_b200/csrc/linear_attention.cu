@@ -152,6 +152,7 @@ scan_kernel(const ScanArgs args) {
                 const int i = e / (kBlock / 4), j0 = e % (kBlock / 4) * 4;
                 if (i >= n || j0 >= n || (REVERSED ? j0 + 3 < i : j0 > i)) continue;
                 float2 s[4] = {};
+#pragma unroll 4
                 for (int k = 0; k < N; k += 4) {
                     const float4 x = *reinterpret_cast<const float4 *>(sa + i * PITCH + k);
 #pragma unroll
@@ -194,10 +195,14 @@ scan_kernel(const ScanArgs args) {
                     float out[R];
 #pragma unroll
                     for (int r = 0; r < R; ++r) out[r] = v[0][r] * f;
-                    for (int j = REVERSED ? i : 0; j <= (REVERSED ? n - 1 : i); ++j) {
+                    const int j_end = REVERSED ? n : i + 1;
+#pragma unroll 4
+                    for (int j = REVERSED ? i : 0; j < j_end; ++j) {
                         const float w = sp[i * kBlock + j];
+                        float cj[R];
+                        ldn(cj, sc + j * PITCH + row0);
 #pragma unroll
-                        for (int r = 0; r < R; ++r) out[r] = fmaf(w, sc[j * PITCH + row0 + r], out[r]);
+                        for (int r = 0; r < R; ++r) out[r] = fmaf(w, cj[r], out[r]);
                     }
                     stn<R>(y + (first + i) * step + row0, out);
                 }
@@ -209,11 +214,13 @@ scan_kernel(const ScanArgs args) {
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int m = 0; m < 8; ++m) S[r][m] = __ffma2_rn(S[r][m], make_float2(dn, dn), __fmul2_rn(S[r][m], make_float2(dl, dl)));
+#pragma unroll 2
         for (int j = 0; j < n; ++j) {
             const float w = dec[REVERSED ? j + 1 : n - 1 - j];
             float cw[R];
+            ldn(cw, sc + j * PITCH + row0);
 #pragma unroll
-            for (int r = 0; r < R; ++r) cw[r] = w * sc[j * PITCH + row0 + r];
+            for (int r = 0; r < R; ++r) cw[r] *= w;
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const float4 x = *reinterpret_cast<const float4 *>(sb + j * PITCH + column(m));
@@ -265,9 +272,9 @@ __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args
     }
 }
 
-// CTAs of a pass that an SM holds, by registers and shared memory, and the blocks that a segment has at the least: two states go through
-// memory for every segment, as much as 96 tokens of fp32 vectors.
-constexpr int64_t kLeastBlocks = 4;
+// CTAs of a pass that an SM holds, by registers and shared memory.  A segment has one block at the least: with four, which spare a state's
+// way through memory for every 64 tokens, 2 x 1000 tokens of 12 heads took 61 us and 300 of 12 heads 48, with one 46 and 20.
+constexpr int64_t kLeastBlocks = 1;
 int64_t places(const LinearAttentionPass &p) { return (int64_t)p.num_sms * (p.N == 128 ? 2 : 8); }
 
 template <typename T, int N>
