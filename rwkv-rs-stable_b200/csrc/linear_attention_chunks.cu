@@ -8,18 +8,18 @@
 //
 //   y_i = sum_{j >= i} d^(j-i) (a_i . b_j) c_j + d^(n-1-i) G a_i      G' = d^n G + sum_j d^(j+1) c_j b_j^T
 //
-// Four products of a chunk: P = A B^T [128 x 128], Y2 = A S [128 x 64], the sum for S' = B^T (w C) [64 x 64] and, once P carries
-// its decays and its mask, Y1 = P C [128 x 64].  A walk over the chunks is bound by HBM (64 KB a chunk, 1.5 us of an SM's share) if
-// two CTAs an SM take at most 3 us for one: so the chunk's chain of waits is kept short.  P stays in TMEM: read as fp32, written
-// back as the bf16 operand of its own product.  Two threads share a row, which halves what is done between two products; c has two
-// buffers, for which the last part of w C takes the place of a as soon as a has been read.
+// Four products of a chunk: P = A B^T [128 x 128], Y2 = A S [128 x 64], the sum for S' = (w C)^T B [64 x 64] and, once P carries
+// its decays and its mask, Y1 = P C [128 x 64].  HBM gives an SM a chunk's 64 KB in 1.5 us.  What is scarcer is shared memory's
+// 128 bytes a cycle, which the products' operands, the loads and everything else share: so P and w C are operands in TMEM.
+// One CTA an SM runs all of it as a pipeline:
+//   warps 0-7         P of a chunk, then y          (two threads a row: a TMEM lane and a half of its columns)
+//   warps 8 9 12 13   w C of the chunk behind, transposed and in three parts, put into TMEM when the product of this one has read the last
+//   warps 16 17       S behind a chunk from its product, one row of S a thread
+//   warp 10           issues the products: the sum for S' (which y of the chunk in front is read beside), P, Y2, Y1
+//   warp 11           loads, four chunks ahead, and stores y from where c was
 //
 // Precision: y is rounded to bf16, and so is P (once); S stays in fp32 registers and enters Y2 as hi + lo (16 bits and a
 // sign), because its errors would add up; the sum for S' takes w C as hi + mid + lo, all 24 bits, because S is an fp32 output.
-//
-// Warps 0-7 own half a row (TMEM lane) a thread, warp 8 issues the products, warp 9 the loads.  The state's rows are those of b, on
-// lanes 0-63 forwards and 64-127 reversed: of the two 64-row blocks of that product's A operand the other one is whatever
-// tile lies beside b, and its lanes are not read.  (So the warps with the smaller share of the triangle P update S.)
 //
 // Entries of c that are not finite would reach tokens on the other side of the mask (0 x inf): a chunk that has some takes
 // them as zero and sets what they do reach, the column's later tokens and the state's column, to NaN.
@@ -34,6 +34,7 @@
 #include "kernels.h"
 #include "launch.h"
 #include "linear_attention_plan.h"
+#include "sm100_mma.cuh"
 #include "sm100_umma.cuh"
 
 namespace rwkv7 {
@@ -42,19 +43,31 @@ namespace {
 using namespace sm100;
 
 constexpr int kN = 64, kL = linear_attention_plan::kChunk;
-constexpr int kRowThreads = 256, kThreads = kRowThreads + 64;
+constexpr int kGroup = 256, kThreads = 576, kStages = 4;
 constexpr uint32_t kTile = kL * 128;           // [128 tokens][64] bf16, 128-byte swizzle
-// Shared memory: a (then the last part of w C), b, c twice (in this order, see above), two parts of w C, S in two, tables, barriers.
-constexpr uint32_t kA = 0, kB = kTile, kC = 2 * kTile, kW = 4 * kTile, kS = 6 * kTile, kSPart = kN * 128;
+// Shared memory: a, b, c of every stage, two parts of S, tables, barriers.
+constexpr uint32_t kA = 0, kB = kTile, kC = 2 * kTile, kStage = 3 * kTile, kS = kStages * kStage, kSPart = kN * 128;
 constexpr uint32_t kCol = kS + 2 * kSPart;     // d^31 .. d^0 forwards, d^0 .. d^31 reversed
-constexpr uint32_t kDec = kCol + 128;          // d^0 .. d^128
+constexpr uint32_t kDiag = kCol + 128;         // the same continued by zeros (reversed: behind zeros), four times, each a word further on
+constexpr uint32_t kDiagWords = 68;
+constexpr uint32_t kDec = kDiag + 4 * kDiagWords * 4;   // d^0 .. d^128
 constexpr uint32_t kBars = kDec + 520;
-constexpr uint32_t kBad = kBars + 120;         // per column the first (reversed: last) token that is not finite
-constexpr uint32_t kSmem = kBad + 256;
-static_assert(kSmem <= 115712, "two CTAs on an SM");
-// TMEM columns: P as fp32 at 0; as bf16 its first half on columns 0-31, its second on 96-127, where the threads that read
-// those columns put it; Y1 between them; Y2 and the state's sum.
-constexpr uint32_t kP = 0, kY1 = 32, kY2 = 128, kKV = 192;
+enum Bar {   // [stage], [parity of the chunk], or one
+    kFull,                                                // a, b and c are loaded
+    kFreeA = kFull + kStages, kFreeB = kFreeA + kStages,  // the last product that reads it is done
+    kYStored = kFreeB + kStages,
+    kAddDone = kYStored + kStages, kAddRead = kAddDone + 2,
+    kPDone = kAddRead + 2, kPReady, kYDone, kYRead, kWReady, kSReady, kEnd, kBarCount
+};
+constexpr uint32_t kSlot = kBars + kBarCount * 8;   // TMEM address, then the last chunk in each stage with entries that are not finite
+// [stage][column]: 128 x chunk + 127 - the first such token (reversed: + the last)
+constexpr uint32_t kBad = kSlot + 24;
+constexpr uint32_t kSmem = kBad + kStages * kN * 4;
+static_assert(kSmem <= 232448, "shared memory of a CTA");
+// TMEM columns.  P as fp32 on 128; as bf16 its first half on columns 0-31, its second on 96-127, where the threads that read those
+// columns put it; Y1 between them.  Y2; the sums for S' of even and odd chunks; three parts of w C (lanes 0-63).
+constexpr uint32_t kP = 0, kY1 = 32, kY2 = 128, kW = 320;
+__host__ __device__ constexpr uint32_t t_add(int it) { return 192 + (it & 1) * 64; }
 __host__ __device__ constexpr uint32_t p_operand(int kstep) { return kP + (kstep < 4 ? 0 : 64) + kstep * 8; }
 
 struct Maps {
@@ -74,26 +87,39 @@ struct ChunkArgs {
     int *status;
 };
 
-enum Bar { kFullA, kFullB, kFullC, kFullC1, kPDone, kADone, kYDone, kKvDone, kSReady, kPReady, kWReady, kYRead, kYStored, kEnd, kBarCount };
-static_assert(kBarCount * 8 + 8 <= 120, "room for the barriers");
-
 // 16-byte piece `q` of a 128-byte row.
 __device__ __forceinline__ uint32_t piece(int row, int q) { return (uint32_t)row * 128u + (uint32_t)((q ^ (row & 7)) << 4); }
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ float2 unpack2(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 __device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf2(v.x, v.y); }
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __fadd2_rn(a, make_float2(-b.x, -b.y)); }
-__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// What is not finite in 16 columns (two pieces) of a token becomes zero, and its place is noted: first + 127 - token (reversed: + token).
+// In loops, as all that is rare or can be: a kernel of several roles lives on what the instruction caches hold of each.  Unrolled, with this for
+// every register, a chunk took 7300 cycles instead of 4400, most of them waits for instructions.
+__device__ __forceinline__ void take_out(unsigned char *tile, int token, int c8, int *bad_from, int first, bool reversed) {
+#pragma unroll 1
+    for (int j = 0; j < 16; ++j) {
+        unsigned short *c = reinterpret_cast<unsigned short *>(tile + piece(token, c8 + j / 8) + j % 8 * 2);
+        if ((*c & 0x7f80) != 0x7f80) continue;
+        *c = 0;
+        atomicMax(bad_from + c8 * 8 + j, first + (reversed ? token : kL - 1 - token));
+    }
+}
+// Half a row of y gets NaN where such an entry reaches it.
+__device__ __forceinline__ void put_nan(unsigned char *tile, int token, int half, const int *bad_from, int first, bool reversed) {
+#pragma unroll 1
+    for (int j = half * 32; j < half * 32 + 32; ++j) {
+        const int from = bad_from[j] - first;   // (negative: of an earlier chunk)
+        if (from >= 0 && (reversed ? token <= from : token >= kL - 1 - from))
+            *reinterpret_cast<unsigned short *>(tile + piece(token, j / 8) + j % 8 * 2) = 0x7fff;
+    }
+}
+
 // ADDS: only what a segment adds to the state.
 template <bool REVERSED, bool ADDS>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
 chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -103,29 +129,38 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     }
     const uint32_t base = smem_u32(smem);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + kBars);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + kBars + kBarCount * 8);
-    float *dec = reinterpret_cast<float *>(smem + kDec), *col = reinterpret_cast<float *>(smem + kCol);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + kSlot);
+    volatile int *bad_chunk = reinterpret_cast<volatile int *>(smem + kSlot + 4);
     int *bad_from = reinterpret_cast<int *>(smem + kBad);
-    volatile int *bad_chunk = reinterpret_cast<volatile int *>(tmem_slot + 1);   // the last chunk with entries that are not finite
-    constexpr uint32_t kColumns = ADDS ? 64 : 256;
+    float *dec = reinterpret_cast<float *>(smem + kDec), *col = reinterpret_cast<float *>(smem + kCol), *diag = reinterpret_cast<float *>(smem + kDiag);
+    constexpr int kMmaWarp = 10, kLoadWarp = 11, kStateWarp = 16;   // (w C and S are on lanes 0-63: their warps are numbers 0 and 1 of four)
     if (tid == 0) {
         for (int i = 0; i < kBarCount; ++i)
-            mbar_init(bar + i, i == kSReady ? 2 * kN : i >= kPReady && i <= kYStored ? kRowThreads : 1);
-        *bad_chunk = -1;
+            mbar_init(bar + i, (i >= kYStored && i < kAddDone) || i == kPReady || i == kYRead ? kGroup
+                               : i == kWReady ? kGroup / 2 : (i >= kAddRead && i < kPDone) || i == kSReady ? kN : i < kFreeA ? (ADDS ? 2 : 3) : 1);
         mbar_fence_init();
+        for (int i = 0; i < kStages; ++i) bad_chunk[i] = -1;
     }
-    if (warp == 8) tmem_alloc(tmem_slot, kColumns);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t t_kv = tmem + (ADDS ? 0 : kKV);
-
+    if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
     wait_for_previous();
     const int chain = blockIdx.x % p.chains, order = blockIdx.x / p.chains;
     const int bi = chain / p.H, h = chain % p.H;
     const int len = p.lens == nullptr ? p.T : min(max(p.lens[bi], 0), p.T);
     const float lambda = p.log_decay[h];
+    // d^k; d^0 is 1 for every d
+    auto power = [&](int k) { return k == 0 ? 1.f : expf(lambda * (float)k); };
+    if (tid <= kL) dec[tid] = power(tid);
+    if (tid >= kGroup && tid < kGroup + 32) col[tid - kGroup] = power(REVERSED ? tid - kGroup : 31 - (tid - kGroup));
+    if (tid >= kGroup && tid < kGroup + kStages * kN) bad_from[tid - kGroup] = -1;
+    // diag[shift][k + shift] for k = e - lane + 31: d^(lane - e) where e <= lane (reversed: d^(e - lane) where e >= lane), else 0
+    for (int i = tid; i < (int)(4 * kDiagWords); i += kThreads) {
+        const int gap = REVERSED ? i % (int)kDiagWords - i / (int)kDiagWords - 31 : 31 - (i % (int)kDiagWords - i / (int)kDiagWords);
+        diag[i] = gap >= 0 && gap < 32 ? power(gap) : 0.f;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
     // The order-th segment that is worked on, its tokens and chunks.
     const int seg = REVERSED ? p.segments - 1 - order : order;
     const int64_t seg_tokens = (int64_t)p.chunks * kL;
@@ -133,160 +168,135 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     const int live = min(len, end) - begin;   // tokens of this segment (none if not positive)
     const int count = live > 0 ? (live + kL - 1) / kL : 0;
     auto first_token = [&](int it) { return begin + (REVERSED ? count - 1 - it : it) * kL; };
-    // d^k; d^0 is 1 for every d
-    auto power = [&](int64_t k) { return k == 0 ? 1.f : expf(lambda * (float)k); };
-    // Rows wait for one another at barriers, so none leaves early: after a time-out a thread waits no more and walks on to the end.
+    auto tokens_of = [&](int it) { return min(kL, len - first_token(it)); };   // all but the sequence's last chunk have 128
+    // A barrier of the chunk's stage, or of its parity, in the chunk's turn of it.  A thread whose wait has run out waits no more, and walks
+    // on to the end, so that nobody waits for it at a barrier of threads.
     bool ok = true;
-    auto wait = [&](Bar b, uint32_t parity) {
+    auto wait = [&](int b, uint32_t parity) {
         if (ok) ok = mbar_wait(bar + b, parity);
+        return ok;
     };
+    auto wait_stage = [&](int b, int it) { return wait(b + it % kStages, (uint32_t)(it / kStages) & 1u); };
+    auto wait_turn = [&](int b, int it) { return wait(b + (it & 1), (uint32_t)(it >> 1) & 1u); };
 
-    if (warp == 9) {
-        // ---- loads: a tile is refilled when the last product that reads it is done
+    if (warp == kLoadWarp) {
+        // ---- loads, and the stores of y
         if (elect_one()) {
-            auto load = [&](int it, const CUtensorMap *map, uint32_t tile, int full) {
-                mbar_expect_tx(bar + full, kTile);
-                tma_load_3d(smem + tile, map, h * kN, first_token(it), bi, bar + full);
-            };
-            auto load_ab = [&](int it) {
+            auto load = [&](int it, const CUtensorMap *map, uint32_t tile) {
                 if (it >= count) return;
-                if (!ADDS) load(it, &maps.a, kA, kFullA);
-                load(it, &maps.b, kB, kFullB);
+                mbar_expect_tx(bar + kFull + it % kStages, kTile);
+                tma_load_3d(smem + it % kStages * kStage + tile, map, h * kN, first_token(it), bi, bar + kFull + it % kStages);
             };
-            auto load_c = [&](int it) {
-                if (it < count) load(it, &maps.c, kC + (it & 1) * kTile, kFullC + (it & 1));
-            };
-            auto prefetch_ab = [&](int it) {   // (their loads have to wait for this chunk's products, and then find them in L2)
-                if (it >= count) return;
-                if (!ADDS) tma_prefetch_3d(&maps.a, h * kN, first_token(it), bi);
-                tma_prefetch_3d(&maps.b, h * kN, first_token(it), bi);
-            };
-            load_ab(0);
-            load_c(0);
-            load_c(1);
-            prefetch_ab(1);
+            for (int it = 0; it < kStages; ++it) {
+                if (!ADDS) load(it, &maps.a, kA);
+                load(it, &maps.b, kB);
+                load(it, &maps.c, kC);
+            }
             for (int it = 0; it < count; ++it) {
-                const uint32_t ph = it & 1;
-                if (it + 1 < count) {
-                    if (!(ok = mbar_wait(bar + kKvDone, ph))) break;
-                    load_ab(it + 1);
-                    prefetch_ab(it + 2);
-                }
-                if (!ADDS) {   // y lies where c was
-                    if (!(ok = mbar_wait(bar + kYStored, ph))) break;
-                    tma_store_3d(&maps.y, h * kN, first_token(it), bi, smem + kC + (it & 1) * kTile);
+                if (!wait_stage(kFreeB, it)) break;
+                load(it + kStages, &maps.b, kB);
+                if (!ADDS) {
+                    if (!wait_stage(kFreeA, it)) break;
+                    load(it + kStages, &maps.a, kA);
+                    if (!wait_stage(kYStored, it)) break;
+                    tma_store_3d(&maps.y, h * kN, first_token(it), bi, smem + it % kStages * kStage + kC);
                     bulk_commit_group();
-                    if (it + 2 < count) bulk_wait_group_read<0>();
+                    if (it + kStages < count) bulk_wait_group_read<0>();
                 }
-                load_c(it + 2);
+                load(it + kStages, &maps.c, kC);
             }
             bulk_wait_group<0>();
-            // (after a time-out what is in flight lands before the CTA leaves: both phases of every tile)
+            // (after a time-out what is in flight lands before the CTA leaves: both phases of every stage)
             if (!ok)
-                for (int tile = kFullA; tile <= kFullC1; ++tile)
-                    for (uint32_t i = 0; i < 2; ++i) mbar_wait(bar + tile, i, 100000u);
+                for (int b = kFull; b < kFreeA; ++b)
+                    for (uint32_t i = 0; i < 2; ++i) mbar_wait(bar + b, i, 100000u);
         }
-    } else if (warp == 8) {
+    } else if (warp == kMmaWarp) {
         // ---- products
         if (elect_one()) {
-            constexpr uint32_t id_p = make_idesc(kFmtBF16, 128, 128, false, false), id_y = make_idesc(kFmtBF16, 128, 64, false, true),
-                               id_kv = make_idesc(kFmtBF16, 128, 64, true, true);
-            // one of the three parts of w C
-            auto add = [&](uint32_t part, bool first) {
-#pragma unroll
-                for (int k = 0; k < kL / 16; ++k)
-                    umma_f16(t_kv, make_smem_desc(base + (REVERSED ? kA : kB) + k * 2048, kTile, 1024),
-                             make_smem_desc(base + part + k * 2048, kTile, 1024), id_kv, !first || k > 0);
-            };
+            constexpr uint32_t id_p = make_idesc(kFmtBF16, 128, 128, false, false), id_y2 = make_idesc(kFmtBF16, 128, 64, false, false),
+                               id_mn = make_idesc(kFmtBF16, 128, 64, false, true);
+            // P first, for what waits for it takes longest; while it is given its decays, the sum for S' and Y2 follow.
             for (int it = 0; it < count; ++it) {
-                const uint32_t ph = it & 1;
+                const uint32_t at = base + it % kStages * kStage, ph = it & 1;
                 if (!ADDS) {
-                    ok = mbar_wait(bar + kFullA, ph) && mbar_wait(bar + kFullB, ph) && (it == 0 || mbar_wait(bar + kYRead, ph ^ 1));
-                    if (!ok) break;
+                    if (!wait_stage(kFull, it) || (it > 0 && !wait(kYRead, ph ^ 1))) break;
                     tc_fence_after();
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
-                        umma_f16(tmem + kP, make_smem_desc(base + kA + k * 32, 16, 1024), make_smem_desc(base + kB + k * 32, 16, 1024), id_p, k > 0);
+                        umma_f16(tmem + kP, make_smem_desc(at + kA + k * 32, 16, 1024), make_smem_desc(at + kB + k * 32, 16, 1024), id_p, k > 0);
                     umma_commit(bar + kPDone);
-                    if (!(ok = mbar_wait(bar + kSReady, ph))) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 2 * (kN / 16); ++k)   // S hi, S lo
-                        umma_f16(tmem + kY2, make_smem_desc(base + kA + (k & 3) * 32, 16, 1024),
-                                 make_smem_desc(base + kS + (k >> 2) * kSPart + (k & 3) * 2048, kSPart, 1024), id_y, k > 0);
-                    umma_commit(bar + kADone);
-                    ok = mbar_wait(bar + kPReady, ph) && mbar_wait(bar + kFullC + (it & 1), (uint32_t)(it >> 1) & 1u);
-                    if (!ok) break;
-                    tc_fence_after();
+                }
+                // (the sum of two chunks ago has been read: S behind it was published before the last Y2)
+                if (!wait(kWReady, ph) || (ADDS && it >= 2 && !wait_turn(kAddRead, it - 2))) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int part = 0; part < 3; ++part)
 #pragma unroll
                     for (int k = 0; k < kL / 16; ++k)
-                        umma_f16_ts(tmem + kY1, tmem + p_operand(k), make_smem_desc(base + kC + (it & 1) * kTile + k * 2048, kTile, 1024), id_y, k > 0);
-                    umma_commit(bar + kYDone);
-                }
-                ok = mbar_wait(bar + kWReady, ph) && (!ADDS || mbar_wait(bar + kFullB, ph));
-                if (!ok) break;
+                        umma_f16_ts(tmem + t_add(it), tmem + kW + part * 64 + k * 8, make_smem_desc(at + kB + k * 2048, kTile, 1024), id_mn, part > 0 || k > 0);
+                umma_commit(bar + kAddDone + ph);
+                umma_commit(bar + kFreeB + it % kStages);
+                if (ADDS) continue;
+                if (!wait(kSReady, ph)) break;
                 tc_fence_after();
-                add(kW, true);
-                add(kW + kTile, false);
-                add(kA, false);
-                umma_commit(bar + kKvDone);
+#pragma unroll
+                for (int k = 0; k < 2 * (kN / 16); ++k)   // S hi, S lo
+                    umma_f16(tmem + kY2, make_smem_desc(at + kA + (k & 3) * 32, 16, 1024),
+                             make_smem_desc(base + kS + (k >> 2) * kSPart + (k & 3) * 32, 16, 1024), id_y2, k > 0);
+                umma_commit(bar + kFreeA + it % kStages);
+                if (!wait(kPReady, ph)) break;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kL / 16; ++k)   // (c is as the products may see it: w C is ready)
+                    umma_f16_ts(tmem + kY1, tmem + p_operand(k), make_smem_desc(at + kC + k * 2048, kTile, 1024), id_mn, k > 0);
+                umma_commit(bar + kYDone);
             }
             umma_commit(bar + kEnd);
             ok = mbar_wait(bar + kEnd, 0) && ok;
         }
-    } else {
-        // ---- rows
-        const int quarter = warp & 3, half = warp >> 2, row = tid & 127;
-        const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
-        const bool has_state = (quarter >= 2) == REVERSED;   // uniform in a warp
-        const int bidx = row & 63, c0 = half * (kN / 2);      // the thread's part of S: row bidx, 32 columns
-        float2 S[kN / 4];
+    } else if (warp >= kStateWarp) {
+        // ---- the state
+        const int row = tid - kStateWarp * 32;   // of S: the thread's column of c
+        const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+        float2 S[kN / 2];
 #pragma unroll
-        for (int j = 0; j < kN / 4; ++j) S[j] = make_float2(0.f, 0.f);
-        if (tid <= kL) dec[tid] = power(tid);
-        if (tid < 32) col[tid] = power(REVERSED ? tid : 31 - tid);
-        constexpr int kNoToken = REVERSED ? -1 : kL;
-        if (tid < kN) bad_from[tid] = kNoToken;
+        for (int j = 0; j < kN / 2; ++j) S[j] = make_float2(0.f, 0.f);
         float *parts = p.parts + (size_t)chain * p.segments * (kN * kN);
         auto write = [&](float *dst) {
 #pragma unroll
-            for (int j = 0; j < kN / 4; ++j) {
-                dst[(c0 + 2 * j) * kN + bidx] = S[j].x;
-                dst[(c0 + 2 * j + 1) * kN + bidx] = S[j].y;
+            for (int j = 0; j < kN / 2; j += 2) *reinterpret_cast<float4 *>(dst + row * kN + 2 * j) = make_float4(S[j].x, S[j].y, S[j + 1].x, S[j + 1].y);
+        };
+        auto read = [&](const float *src, bool transposed) {
+            if (!transposed) {
+#pragma unroll
+                for (int j = 0; j < kN / 2; j += 2) {
+                    const float4 v = *reinterpret_cast<const float4 *>(src + row * kN + 2 * j);
+                    S[j] = make_float2(v.x, v.y);
+                    S[j + 1] = make_float2(v.z, v.w);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN / 2; ++j) S[j] = make_float2(src[2 * j * kN + row], src[(2 * j + 1) * kN + row]);
             }
         };
-        if (has_state) {
-            auto read = [&](const float *src, bool transposed) {
-                if (transposed) {
+        const float *s_in = p.s_in == nullptr ? nullptr : p.s_in + (size_t)chain * (kN * kN);
+        if (ADDS) {
+            if (order == 0) {   // the state in front of everything: s_in may be overwritten before the last segment starts
+                if (s_in != nullptr) read(s_in, p.s_in_transposed);
+                write(parts);
 #pragma unroll
-                    for (int j = 0; j < kN / 4; j += 2) {
-                        const float4 v = *reinterpret_cast<const float4 *>(src + bidx * kN + c0 + 2 * j);
-                        S[j] = make_float2(v.x, v.y);
-                        S[j + 1] = make_float2(v.z, v.w);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kN / 4; ++j) S[j] = make_float2(src[(c0 + 2 * j) * kN + bidx], src[(c0 + 2 * j + 1) * kN + bidx]);
-                }
-            };
-            const float *s_in = p.s_in == nullptr ? nullptr : p.s_in + (size_t)chain * (kN * kN);
-            if (ADDS) {
-                if (order == 0) {   // the state in front of everything: s_in may be overwritten before the last segment starts
-                    if (s_in != nullptr) read(s_in, p.s_in_transposed);
-                    write(parts);
-#pragma unroll
-                    for (int j = 0; j < kN / 4; ++j) S[j] = make_float2(0.f, 0.f);
-                }
-            } else if (p.segments > 1) {
-                read(parts + (size_t)order * (kN * kN), false);
-            } else if (s_in != nullptr) {
-                read(s_in, p.s_in_transposed);
+                for (int j = 0; j < kN / 2; ++j) S[j] = make_float2(0.f, 0.f);
             }
+        } else if (p.segments > 1) {
+            read(parts + (size_t)order * (kN * kN), false);
+        } else if (s_in != nullptr) {
+            read(s_in, p.s_in_transposed);
         }
-        // S as the operand of the next chunk's Y2: row b, columns c, hi and lo
+        // S as the operand of a chunk's Y2: row c, columns b, hi and lo
         auto publish = [&] {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 8; ++q) {
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -294,61 +304,126 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                     hi[e] = pack2(s);
                     lo[e] = pack2(sub2(s, unpack2(hi[e])));
                 }
-                sts16(base + kS + piece(bidx, half * 4 + q), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                sts16(base + kS + kSPart + piece(bidx, half * 4 + q), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                sts16(base + kS + piece(row, q), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                sts16(base + kS + kSPart + piece(row, q), make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
             fence_proxy_async();
             mbar_arrive(bar + kSReady);
         };
-        if (!ADDS && has_state && count > 0) publish();
-        rows_sync();   // (the tables)
-
         for (int it = 0; it < count; ++it) {
-            const uint32_t ph = it & 1, tile_c = kC + (it & 1) * kTile;
-            const int t0 = first_token(it), n = min(kL, len - t0);   // tokens of the chunk: all but the sequence's last have 128
-            uint32_t own[4];   // where this thread's half row lies in a tile
-#pragma unroll
-            for (int q = 0; q < 4; ++q) own[q] = piece(row, half * 4 + q);
-
-            // c as the products may see it
-            wait((Bar)(kFullC + (it & 1)), (uint32_t)(it >> 1) & 1u);
-            if (n < kL) {   // (uniform) behind the sequence anything may stand
-                wait(kFullB, ph);
-                if (row >= n) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        sts16(base + kB + own[q], make_uint4(0u, 0u, 0u, 0u));
-                        sts16(base + tile_c + own[q], make_uint4(0u, 0u, 0u, 0u));
-                    }
-                    fence_proxy_async();
-                }
-            }
-            {
-                uint4 in[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) in[q] = lds16(base + tile_c + own[q]);
-                uint32_t all = 0;   // sign bits: an exponent of ones in the low or the high half of a word
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    for (uint32_t u : {in[q].x, in[q].y, in[q].z, in[q].w}) all |= ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                if (all != 0u) {
-                    for (int j = c0; j < c0 + kN / 2; ++j) {
-                        unsigned short *c = reinterpret_cast<unsigned short *>(smem + tile_c + piece(row, j >> 3) + (j & 7) * 2);
-                        if ((*c & 0x7f80) != 0x7f80) continue;
-                        *c = 0;
-                        if (REVERSED) atomicMax(bad_from + j, row);
-                        else atomicMin(bad_from + j, row);
-                    }
-                    *bad_chunk = it;
-                    fence_proxy_async();
-                }
-            }
-
             if (!ADDS) {
-                // P: decays and mask, and bf16.  Each warp takes two blocks of 32 columns, the outer one first (see p_operand).
-                wait(kPDone, ph);
-                tc_fence_after();
+                if (it > 0) wait_stage(kFreeA, it - 1);   // the Y2 that reads the last one is done
+                publish();
+            }
+            wait_turn(kAddDone, it);
+            tc_fence_after();
+            float dn = dec[tokens_of(it)];
+            if (bad_chunk[it % kStages] == it && bad_from[it % kStages * kN + row] >= it * kL) dn = __uint_as_float(0x7fffffffu);
 #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t v[16];
+                tmem_ld16(tmem + t_add(it) + t_lane + q * 16, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    S[q * 8 + e] = __ffma2_rn(S[q * 8 + e], make_float2(dn, dn), make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])));
+            }
+            tc_fence_before();
+            mbar_arrive(bar + kAddRead + (it & 1));
+        }
+        if (ok && ADDS) write(parts + (size_t)(order + 1) * (kN * kN));
+        if (ok && !ADDS && order == p.segments - 1 && p.s_out != nullptr) write(p.s_out + (size_t)chain * (kN * kN));
+    } else if (warp >= 8 && (warp & 2) == 0) {
+        // ---- w C, transposed and in three parts: 32 columns of c (TMEM lanes) and 64 tokens a warp, in fragments of 8 x 8: a register holds
+        // tokens t and t + 1 of a column, two registers columns eight apart
+        const int quarter = warp & 1, token0 = (warp >> 2 & 1) * 64;
+        const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
+        const int q = lane & 3;
+        // the weights of this lane's pairs of tokens, token0 + 8 i + 2 q and the next, of a chunk of n
+        float2 w[8];
+        auto weigh = [&](int n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = token0 + 8 * i + 2 * q;   // (behind the sequence c is zero)
+                w[i] = make_float2(dec[REVERSED ? t + 1 : max(n - 1 - t, 0)], dec[REVERSED ? t + 2 : max(n - 2 - t, 0)]);
+            }
+        };
+        weigh(kL);
+        for (int it = 0; it < count; ++it) {
+            const int stage = it % kStages, n = tokens_of(it);
+            const uint32_t tile_b = stage * kStage + kB, tile_c = stage * kStage + kC;
+            wait_stage(kFull, it);
+            if (n < kL) {   // (uniform) behind the sequence anything may stand
+#pragma unroll 1
+                for (int i = lane; i < 64 * 4; i += 32) {
+                    const int t = token0 + i / 4;
+                    if (t < n) continue;
+                    sts16(base + tile_b + piece(t, quarter * 4 + i % 4), make_uint4(0u, 0u, 0u, 0u));
+                    sts16(base + tile_c + piece(t, quarter * 4 + i % 4), make_uint4(0u, 0u, 0u, 0u));
+                }
+                __syncwarp();
+            }
+            if (!REVERSED && (n < kL || (it > 0 && tokens_of(it - 1) < kL))) weigh(n);
+#pragma unroll 1
+            for (int side = 0; side < 2; ++side) {   // sixteen columns (lanes) at a time
+                // sixteen tokens: matrices (tokens, columns), (tokens, columns + 8), (tokens + 8, ..), (tokens + 8, .. + 8)
+                const uint32_t src = base + tile_c + piece(token0 + (lane & 7) + (lane >> 4) * 8, quarter * 4 + side * 2 + (lane >> 3 & 1));
+                uint32_t in[4][4];
+                do {
+                    uint32_t not_finite = 0;   // sign bits: an exponent of ones in the low or the high half of a word
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ldsm4_t(in[i], src + i * 16 * 128);   // (sixteen rows on, the swizzle is the same)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) not_finite |= ((in[i][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                    }
+                    if (!__any_sync(0xffffffffu, not_finite != 0)) break;
+                    for (int t = token0 + lane; t < token0 + 64; t += 32)
+                        take_out(smem + tile_c, t, quarter * 4 + side * 2, bad_from + stage * kN, it * kL, REVERSED);
+                    bad_chunk[stage] = it;
+                    __syncwarp();
+                } while (true);
+                uint32_t hi[2][8], mid[2][8], lo[2][8];   // of 32 tokens each
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = i % 4 * 2 + e;
+                        float2 x = __fmul2_rn(unpack2(in[i / 2][i % 2 * 2 + e]), w[i]);
+                        hi[i / 4][r] = pack2(x);
+                        x = sub2(x, unpack2(hi[i / 4][r]));
+                        mid[i / 4][r] = pack2(x);
+                        lo[i / 4][r] = pack2(sub2(x, unpack2(mid[i / 4][r])));
+                    }
+                }
+                if (side == 0 && it > 0) {   // the product that reads the last one's is done
+                    wait_turn(kAddDone, it - 1);
+                    tc_fence_after();
+                }
+                const uint32_t at = tmem + kW + t_lane + ((uint32_t)(side * 16) << 16) + token0 / 2;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    tmem_st_fragments(at + i * 16, hi[i]);
+                    tmem_st_fragments(at + 64 + i * 16, mid[i]);
+                    tmem_st_fragments(at + 128 + i * 16, lo[i]);
+                }
+            }
+            tmem_st_wait();
+            fence_proxy_async();
+            tc_fence_before();
+            mbar_arrive(bar + kWReady);
+        }
+    } else if (!ADDS && warp < 8) {
+        // ---- P of a chunk, then y
+        const int quarter = warp & 3, half = warp >> 2, row = tid & 127, c0 = half * (kN / 2);
+        const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
+        for (int it = 0; it < count; ++it) {
+            const int n = tokens_of(it);
+            {
+                // Each warp takes two blocks of 32 columns, the outer one first (see p_operand).
+                wait(kPDone, it & 1);
+                tc_fence_after();
+#pragma unroll 1
                 for (int i = 0; i < 2; ++i) {
                     const int c = half == 0 ? i : 3 - i;
                     uint32_t out[16];
@@ -360,15 +435,18 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                         tmem_ld32(tmem + kP + t_lane + c * 32, v);
                         tmem_ld_wait();
                         if (c == quarter) {
-                            const float *gap0 = dec + (REVERSED ? -lane : lane);
+                            // lane's factors from word 31 - lane on, in the copy where they start on 16 bytes
+                            const int shift = (lane + 1) & 3;
+                            const float4 *factor = reinterpret_cast<const float4 *>(diag + shift * kDiagWords + 31 - lane + shift);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const bool seen = REVERSED ? e >= lane : e <= lane;
-                                const float g = seen ? gap0[REVERSED ? e : -e] : 0.f;
-                                v[e] = seen ? __float_as_uint(__uint_as_float(v[e]) * g) : 0u;
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 g = factor[e / 4];
+                                const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), make_float2(g.x, g.y));
+                                const float2 z = __fmul2_rn(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), make_float2(g.z, g.w));
+                                auto seen = [&](int j, float r) { return (REVERSED ? j >= lane : j <= lane) ? r : 0.f; };   // (whatever was there)
+                                out[e / 2] = pack_bf2(seen(e, x.x), seen(e + 1, x.y));
+                                out[e / 2 + 1] = pack_bf2(seen(e + 2, z.x), seen(e + 3, z.y));
                             }
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) out[e] = pack_bf2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
                         } else {
                             // d^gap as a factor of the row and one of the column, neither with a negative power
                             const float f = dec[REVERSED ? 32 * c - row : row - 32 * c - 31];
@@ -395,121 +473,46 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 tc_fence_before();
                 mbar_arrive(bar + kPReady);
             }
-
-            // w C in three parts.  (The product that read the previous ones is done, and a has been read.)
-            if (it > 0) wait(kKvDone, ph ^ 1);
-            if (!ADDS) wait(kADone, ph);
-            {
-                const float w = row < n ? dec[REVERSED ? row + 1 : n - 1 - row] : 0.f;
-                uint4 in[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) in[q] = lds16(base + tile_c + own[q]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t u[4] = {in[q].x, in[q].y, in[q].z, in[q].w};
-                    uint32_t hi[4], mid[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float2 x = __fmul2_rn(unpack2(u[e]), make_float2(w, w));
-                        hi[e] = pack2(x);
-                        x = sub2(x, unpack2(hi[e]));
-                        mid[e] = pack2(x);
-                        lo[e] = pack2(sub2(x, unpack2(mid[e])));
-                    }
-                    sts16(base + kW + own[q], make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                    sts16(base + kW + kTile + own[q], make_uint4(mid[0], mid[1], mid[2], mid[3]));
-                    sts16(base + kA + own[q], make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                }
-            }
-            fence_proxy_async();
-            mbar_arrive(bar + kWReady);
-
-            bool any_bad = false;   // (the same for all: every thread has looked at c before the products that are waited for)
-            if (!ADDS) {
-                // y, to where this thread's c was
-                wait(kYDone, ph);
-                tc_fence_after();
-                any_bad = *bad_chunk == it;
-                const float f = dec[REVERSED ? max(n - 1 - row, 0) : row + 1];
-#pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    uint32_t v[16], u[16];
-                    tmem_ld16(tmem + kY1 + t_lane + c0 + part * 16, v);
-                    tmem_ld16(tmem + kY2 + t_lane + c0 + part * 16, u);
-                    tmem_ld_wait();
-                    if (part == 1) {
-                        tc_fence_before();
-                        mbar_arrive(bar + kYRead);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), make_float2(f, f),
-                                                    make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                        u[e / 2] = pack2(x);
-                    }
-                    if (any_bad) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int from = bad_from[c0 + part * 16 + e];
-                            if (REVERSED ? row <= from : row >= from) u[e / 2] |= e & 1 ? 0x7fff0000u : 0x7fffu;
-                        }
-                    }
-                    if (row >= n) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) u[e] = 0u;
-                    }
-                    sts16(base + tile_c + own[2 * part], make_uint4(u[0], u[1], u[2], u[3]));
-                    sts16(base + tile_c + own[2 * part + 1], make_uint4(u[4], u[5], u[6], u[7]));
-                }
-                fence_proxy_async();
-                mbar_arrive(bar + kYStored);
-            }
-            if (has_state) {
-                wait(kKvDone, ph);
-                tc_fence_after();
-                any_bad = *bad_chunk == it;
-                const float dn = dec[n];
-                uint32_t v[32];
-                tmem_ld32(t_kv + t_lane + c0, v);
+            wait(kYDone, it & 1);
+            tc_fence_after();
+            const uint32_t tile_c = it % kStages * kStage + kC;
+            const float f = dec[REVERSED ? max(n - 1 - row, 0) : row + 1];
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+                uint32_t v[16], u[16];
+                tmem_ld16(tmem + kY1 + t_lane + c0 + part * 16, v);
+                tmem_ld16(tmem + kY2 + t_lane + c0 + part * 16, u);
                 tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < kN / 4; ++j)
-                    S[j] = __ffma2_rn(S[j], make_float2(dn, dn), make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])));
-                if (any_bad) {
-#pragma unroll
-                    for (int j = 0; j < kN / 4; ++j) {
-                        if ((unsigned)bad_from[c0 + 2 * j] < (unsigned)kL) S[j].x = __uint_as_float(0x7fffffffu);
-                        if ((unsigned)bad_from[c0 + 2 * j + 1] < (unsigned)kL) S[j].y = __uint_as_float(0x7fffffffu);
-                    }
+                if (part == 1) {
+                    tc_fence_before();
+                    mbar_arrive(bar + kYRead);
                 }
-                tc_fence_before();
-                if (!ADDS && it + 1 < count) publish();
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), make_float2(f, f),
+                                                make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                    u[e / 2] = pack2(x);
+                }
+                if (row >= n) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[e] = 0u;
+                }
+                sts16(base + tile_c + piece(row, half * 4 + 2 * part), make_uint4(u[0], u[1], u[2], u[3]));
+                sts16(base + tile_c + piece(row, half * 4 + 2 * part + 1), make_uint4(u[4], u[5], u[6], u[7]));
             }
-            if (ADDS) {
-                wait(kKvDone, ph);
-                any_bad = *bad_chunk == it;
-            }
-            if (any_bad) {
-                rows_sync();   // (all have read it)
-                if (tid < kN) bad_from[tid] = kNoToken;
-                rows_sync();
-            }
+            if (bad_chunk[it % kStages] == it && row < n) put_nan(smem + tile_c, row, half, bad_from + it % kStages * kN, it * kL, REVERSED);
+            fence_proxy_async();
+            mbar_arrive(bar + kYStored + it % kStages);
         }
-        if (ok && !ADDS) {   // chunks behind the sequence
-            const int from = begin + count * kL;
-            for (int64_t i = tid; i < (int64_t)(end - from) * 8; i += kRowThreads)
-                *reinterpret_cast<uint4 *>(p.y + (((int64_t)bi * p.T + from + i / 8) * p.H + h) * kN + i % 8 * 8) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        if (ok && has_state) {
-            if (ADDS) write(parts + (size_t)(order + 1) * (kN * kN));
-            else if (order == p.segments - 1 && p.s_out != nullptr) write(p.s_out + (size_t)chain * (kN * kN));
-        }
+        const int from = begin + count * kL;   // chunks behind the sequence
+        for (int64_t i = tid; ok && i < (int64_t)(end - from) * 8; i += kGroup)
+            *reinterpret_cast<uint4 *>(p.y + (((int64_t)bi * p.T + from + i / 8) * p.H + h) * kN + i % 8 * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
     __syncwarp();
     if (!ok) atomicExch(p.status, (int)kDevTimeout);
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem, kColumns);
+    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,

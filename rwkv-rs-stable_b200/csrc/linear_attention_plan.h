@@ -14,7 +14,7 @@ namespace rwkv7 {
 namespace linear_attention_plan {
 
 constexpr int kChunk = 128;   // tokens of a chunk of the tensor-core kernel
-constexpr int kResident = 2;  // its CTAs per SM
+constexpr int kResident = 1;  // its CTAs per SM
 constexpr int kBlock = 16;    // tokens of a block of the other kernel
 
 struct Cut {
