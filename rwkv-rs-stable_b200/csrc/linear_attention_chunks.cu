@@ -141,26 +141,32 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         mbar_fence_init();
         for (int i = 0; i < kStages; ++i) bad_chunk[i] = -1;
     }
-    if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
-    wait_for_previous();
-    const int chain = blockIdx.x % p.chains, order = blockIdx.x / p.chains;
-    const int bi = chain / p.H, h = chain % p.H;
-    const int len = p.lens == nullptr ? p.T : min(max(p.lens[bi], 0), p.T);
-    const float lambda = p.log_decay[h];
-    // d^k; d^0 is 1 for every d
-    auto power = [&](int k) { return k == 0 ? 1.f : expf(lambda * (float)k); };
-    if (tid <= kL) dec[tid] = power(tid);
-    if (tid >= kGroup && tid < kGroup + 32) col[tid - kGroup] = power(REVERSED ? tid - kGroup : 31 - (tid - kGroup));
     if (tid >= kGroup && tid < kGroup + kStages * kN) bad_from[tid - kGroup] = -1;
-    // diag[shift][k + shift] for k = e - lane + 31: d^(lane - e) where e <= lane (reversed: d^(e - lane) where e >= lane), else 0
-    for (int i = tid; i < (int)(4 * kDiagWords); i += kThreads) {
-        const int gap = REVERSED ? i % (int)kDiagWords - i / (int)kDiagWords - 31 : 31 - (i % (int)kDiagWords - i / (int)kDiagWords);
-        diag[i] = gap >= 0 && gap < 32 ? power(gap) : 0.f;
-    }
+    if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();
+    const int chain = blockIdx.x % p.chains, order = blockIdx.x / p.chains;
+    const int bi = chain / p.H, h = chain % p.H;
+    const int len = p.lens == nullptr ? p.T : min(max(p.lens[bi], 0), p.T);
+    // Tables, by those that use them; the loads start meanwhile.
+    if (warp != kMmaWarp && warp != kLoadWarp) {
+        const float lambda = p.log_decay[h];
+        auto power = [&](int k) { return k == 0 ? 1.f : expf(lambda * (float)k); };   // d^k; d^0 is 1 for every d
+        if (tid <= kL) dec[tid] = power(tid);
+        const int other = (tid < kMmaWarp * 32 ? tid : tid - 64) - (kL + 1);   // threads that have no entry of dec
+        if (other >= 0 && other < 32) col[other] = power(REVERSED ? other : 31 - other);
+        // diag[shift][k + shift] for k = e - lane + 31: d^(lane - e) where e <= lane (reversed: d^(e - lane) where e >= lane), else 0
+        const int i = other - 32;
+        static_assert(kThreads - 64 - (kL + 1) - 32 >= (int)(4 * kDiagWords));
+        if (i >= 0 && i < (int)(4 * kDiagWords)) {
+            const int gap = REVERSED ? i % (int)kDiagWords - i / (int)kDiagWords - 31 : 31 - (i % (int)kDiagWords - i / (int)kDiagWords);
+            diag[i] = gap >= 0 && gap < 32 ? power(gap) : 0.f;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 64) : "memory");
+    }
     // The order-th segment that is worked on, its tokens and chunks.
     const int seg = REVERSED ? p.segments - 1 - order : order;
     const int64_t seg_tokens = (int64_t)p.chunks * kL;

@@ -58,6 +58,29 @@ def test_forward(pkg, cuda, B, T, H, N, dtype):
     _check_forward(pkg, _inputs(cuda, B, T, H, N, dtype, seed=T)[0], dtype)
 
 
+@pytest.mark.parametrize("T,ragged", [(64, False), (130, True), (300, True), (1100, True)])
+def test_more_chains_than_the_device_holds(pkg, cuda, T, ragged):
+    """Short sequences: a CTA goes over several chains, some without a token; longer ones: more CTAs than SMs.  Every chain has its own
+    decay, state and length."""
+    B, H = 60, 9
+    lens = [(37 * b) % (T + 1) if ragged else T for b in range(B)]
+    x, dy, ds = _inputs(cuda, B, T, H, 64, BF16, seed=T, lens=lens)
+    for t in (x["q"], x["k"], x["v"], dy):
+        for b, e in enumerate(lens):
+            t[b, e:] = float("nan")
+    _check_forward(pkg, x, BF16)
+    inputs = pkg.LinearAttentionForwardInputs(x["q"], x["k"], x["v"], x["log_decay"], context_lens=x["lens"])
+    grads, ds0 = pkg.linear_attention_backward(inputs, dy, ds, initial_state=x["s0"])
+    dy0 = torch.nan_to_num(dy, nan=0.0)
+    for part in (slice(0, 20), slice(20, 40), slice(40, 60)):   # (the 64-bit form takes every pair of tokens at once)
+        y = {n: t if n == "log_decay" else t[part] for n, t in x.items()}
+        want = ref.attention_grads(**y, dy=dy0[part], ds=ds[part])
+        mag = ref.attention_grads(**_abs(y), dy=dy0[part].abs(), ds=ds[part].abs())
+        for name, got, w, m in zip(("query", "key", "value", "state"), (*grads, ds0), want, mag):
+            _close(got[part], w, m, T, 64, BF16, name)
+    assert pkg.read_device_status(0) == 0
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("T", [1, 31, 200])
 def test_zero_state_and_no_state_wanted(pkg, cuda, T, dtype):
