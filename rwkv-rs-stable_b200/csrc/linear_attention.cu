@@ -272,9 +272,7 @@ __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args
     }
 }
 
-// CTAs of a pass that an SM holds, by registers and shared memory.  A segment has one block at the least: with four, which spare a state's
-// way through memory for every 64 tokens, 2 x 1000 tokens of 12 heads took 61 us and 300 of 12 heads 48, with one 46 and 20.
-constexpr int64_t kLeastBlocks = 1;
+// CTAs of a pass that an SM holds, by registers and shared memory.
 int64_t places(const LinearAttentionPass &p) { return (int64_t)p.num_sms * (p.N == 128 ? 2 : 8); }
 
 template <typename T, int N>
@@ -314,14 +312,14 @@ size_t linear_attention_workspace_bytes(const LinearAttentionPass &p) {
     using namespace linear_attention_plan;
     if (linear_attention_chunks_supported(p)) return linear_attention_chunks_workspace_bytes(p);
     const int64_t chains = p.B * p.H;
-    return state_bytes(chains, cut(chains, (p.T + kBlock - 1) / kBlock, places(p), kLeastBlocks, INT64_MAX).segments, p.N);
+    return state_bytes(chains, cut(chains, (p.T + kBlock - 1) / kBlock, places(p), kBlocksOfLaunches, INT64_MAX).segments, p.N);
 }
 
 int launch_linear_attention(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
     using namespace linear_attention_plan;
     if (linear_attention_chunks_supported(p)) return launch_linear_attention_chunks(p, workspace, workspace_bytes, stream);
     const int64_t chains = p.B * p.H;
-    const Cut c = cut(chains, (p.T + kBlock - 1) / kBlock, places(p), kLeastBlocks, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, p.N));
+    const Cut c = cut(chains, (p.T + kBlock - 1) / kBlock, places(p), kBlocksOfLaunches, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, p.N));
     const ScanArgs args{p, c.segments > 1 ? static_cast<float *>(workspace) : nullptr, c.segments, c.chunks * kBlock};
     return p.bf16 ? launch_scan<__nv_bfloat16>(args, stream) : launch_scan<float>(args, stream);
 }

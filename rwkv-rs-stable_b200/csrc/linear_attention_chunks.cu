@@ -562,18 +562,23 @@ cudaError_t launch(const Maps &maps, const ChunkArgs &args, int64_t ctas, int de
 
 }  // namespace
 
-bool linear_attention_chunks_supported(const LinearAttentionPass &p) { return p.bf16 && p.N == kN && p.T >= 64; }
+// A chunk takes a CTA about 6.5 us whatever it holds, one CTA an SM; the other kernel's blocks of sixteen tokens share the SMs.  Prompts of 17, 32
+// and 48 tokens, this kernel and the other: 128 chains 8.6, 8.5, 7.5 and 9.5, 13.5, 20.4 us; 384 chains 20.1, 20.3, 20.7 and 12.3, 17.9, 22.1 (of 40);
+// 768 chains 37.7, 37.5, 37.9 and 17.6, 25.9, 36.6.
+bool linear_attention_chunks_supported(const LinearAttentionPass &p) {
+    return p.bf16 && p.N == kN && (p.T >= 48 || (p.T > linear_attention_plan::kBlock && p.B * p.H <= p.num_sms));
+}
 
 size_t linear_attention_chunks_workspace_bytes(const LinearAttentionPass &p) {
     using namespace linear_attention_plan;
     const int64_t chains = p.B * p.H;
-    return state_bytes(chains, cut(chains, (p.T + kL - 1) / kL, (int64_t)p.num_sms * kResident, 1, INT64_MAX).segments, kN);
+    return state_bytes(chains, cut(chains, (p.T + kL - 1) / kL, (int64_t)p.num_sms, kChunksOfLaunches, INT64_MAX).segments, kN);
 }
 
 int launch_linear_attention_chunks(const LinearAttentionPass &p, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
     using namespace linear_attention_plan;
     const int64_t chains = p.B * p.H;
-    const Cut c = cut(chains, (p.T + kL - 1) / kL, (int64_t)p.num_sms * kResident, 1, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, kN));
+    const Cut c = cut(chains, (p.T + kL - 1) / kL, (int64_t)p.num_sms, kChunksOfLaunches, workspace == nullptr ? 1 : segments_in(workspace_bytes, chains, kN));
     Maps maps;
     if (!describe(&maps.a, p.a, p) || !describe(&maps.b, p.b, p) || !describe(&maps.c, p.c, p) || !describe(&maps.y, p.y, p)) return (int)cudaErrorInvalidValue;
     ChunkArgs args{};
