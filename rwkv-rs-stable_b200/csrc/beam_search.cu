@@ -2,10 +2,12 @@
 //
 // A candidate (i, t) of a search is token t behind beam i, with score[i] + x[i][t] - log sum_t exp x[i][t].  The first kernel
 // goes once over the beams' rows: the maximum, the sum of exponentials and the K largest logits, among which are all that can be chosen.
-// It is bound by the bytes of the logits, and nearly by its instructions: five a logit (unpack, maximum, scale, exponential,
-// sum).  So nothing else is done to most of them: a bound under the K-th largest is known, the K-th largest of the threads' maxima of
-// some 8192 logits, which at least K reach and hardly more, and only a thread whose maximum reaches it puts its logits aside; those are
-// gone through from time to time, by all threads.  The second kernel takes the K best of a search from its rows' sorted lists.
+// Its floor is the bytes of the logits; it is bound by its instructions, some seven a logit (unpack, maximum, scale, exponential, sum and
+// their surroundings).  So nothing else is done to most of them: a bound under the K-th largest is known, the K-th largest of the threads'
+// maxima of some 8192 logits, which at least K reach and hardly more, and only a thread whose maximum reaches it puts its logits aside; those
+// are gone through from time to time, by all threads, and the bound is raised to the K-th largest of what was kept.  512 rows of 65536 bf16,
+// K = 8: 24 us, 10.2 by its bytes (27.8 where the bound stayed where it was).  The second kernel takes the K best of a search from its
+// rows' sorted lists; four rows of 65536 fp32 take both kernels 7.3 us (13.5 with every list's head ranked against every other's).
 // Scores are compared in 64 bits: the candidates of different beams lie as close together as their last bits, and a 32-bit score in
 // the tens has only four decimals behind the point.  Ties go to the lowest i V + t.  A logit that is NaN counts as -inf, +inf as the
 // largest finite number.
@@ -59,8 +61,8 @@ __device__ C block_first(C c, C *shared) {
 }
 
 constexpr int kVectors = 4;                          // 16-byte vectors a thread has in registers, and as many on their way
-constexpr int kMostAside = kThreads + 64;            // threads' vectors put aside: gone through when there are more than 64
-constexpr int kMostKept = 2048, kMany = 512;         // logits over the bound: room for, and when to raise it
+constexpr int kMostAside = kThreads + 32;            // threads' vectors put aside: gone through when there are more than 32
+constexpr int kMostKept = 2048;                      // logits over the bound: room for; it is raised when they are many for K
 constexpr int kMostSplits = 32;                      // CTAs on a row
 
 // Pieces of a row.  They start on 16 bytes, the first at or (where rows are not whole vectors) before the row's start.
@@ -119,7 +121,7 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
     wait_for_previous();
     let_next_in();
     const T *logits = static_cast<const T *>(p.logits);
-    const int64_t begin = row * p.V, end = begin + p.V, all = p.B * p.I * p.V;
+    const int64_t begin = row * p.V, end = begin + p.V;
     const int64_t base = begin / VEC * VEC;
     const int V = (int)p.V;
 
@@ -176,7 +178,7 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
         }
         __syncthreads();
         if (tid == 0) n_aside = 0;
-        if (n_kept > kMany) {
+        if (n_kept > 2 * p.K + 16) {
             const int n = min(n_kept, kMostKept);
             slow = slow || n_kept > kMostKept;
             for (int i = tid; i < n; i += kThreads) {
@@ -339,9 +341,6 @@ struct Choice {
     int beam, token;
 };
 __device__ constexpr Choice kNoChoice{0, INT_MAX, INT_MAX};
-__device__ __forceinline__ bool before(const Choice &a, const Choice &b) {
-    return a.score > b.score || (a.score == b.score && (a.beam < b.beam || (a.beam == b.beam && a.token < b.token)));
-}
 
 // One search: the K first of its sorted lists, one of every split of every beam.  They come from the K lists with the first heads, which
 // are at most 32: one warp, a list a lane, takes the first of all heads K times.
@@ -350,11 +349,20 @@ beam_merge_kernel(const BeamSelectArgs p, int splits, const float2 *sums, const 
     __shared__ double log_sum[32];   // of a row, behind its maximum
     __shared__ float top[32];
     __shared__ Choice heads[32 * kMostSplits], lists_of[32][32];
-    __shared__ int chosen[32];
+    __shared__ uint64_t ranked[32 * kMostSplits];   // heads that may be among the first, in any order
+    __shared__ int ranked_list[32 * kMostSplits], n_ranked, chosen[32];
+    __shared__ uint32_t tops[kWarps][32];
     const int64_t search = blockIdx.x, first = search * p.I;
     const int lists = p.I * splits, tid = threadIdx.x;
+    if (tid == 0) n_ranked = 0;
     wait_for_previous();
-    {   // eight lanes a row
+    // A list's entry is asked for before what its row adds to it is known.
+    auto entry = [&](int l, int k) {
+        const int64_t at = (first * splits + l) * p.K + k;
+        return Candidate<float, int>{values[at], tokens[at]};
+    };
+    const Candidate<float, int> mine = tid < lists ? entry(tid, 0) : Candidate<float, int>{0.f, -1};
+    {   // eight lanes a row.  The parts' sums are good to 32 bits, and so are the factors; the sum of sums and its logarithm have 64.
         const int i = tid >> 3, lane = tid & 7;
         float2 s[kMostSplits / 8];
         float most = -INFINITY;
@@ -368,20 +376,22 @@ beam_merge_kernel(const BeamSelectArgs p, int splits, const float2 *sums, const 
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < kMostSplits / 8; ++j)
-            if (s[j].y > 0.f) sum += s[j].x == most ? (double)s[j].y : (double)s[j].y * exp((double)s[j].x - (double)most);
+            if (s[j].y > 0.f) sum += (double)(s[j].y * expf(s[j].x - most));
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (i < p.I && lane == 0) {
             top[i] = most;
-            log_sum[i] = log(sum);
+            log_sum[i] = sum;
         }
     }
     __syncthreads();
-    auto candidate = [&](int l, int k) {
+    if (tid < p.I) log_sum[tid] = log(log_sum[tid]);   // (one warp: a double's logarithm is long)
+    __syncthreads();
+    auto candidate = [&](int l, int k, Candidate<float, int> c) {
         const int i = l / splits;
-        const int64_t row = first + i, at = (first * splits + l) * p.K + k;
-        const float score = clean(p.scores[row]), x = values[at];
-        const int token = tokens[at];
+        const int64_t row = first + i;
+        const float score = clean(p.scores[row]), x = c.value;
+        const int token = c.index;
         const bool finished = p.finished != nullptr && p.finished[row] != 0;
         if (score == -INFINITY || finished) {
             // -inf whatever the logits; finished: the padding token at no cost, and nothing else
@@ -393,23 +403,43 @@ beam_merge_kernel(const BeamSelectArgs p, int splits, const float2 *sums, const 
         const double lp = x == -INFINITY ? -INFINITY : ((double)x - (double)top[i]) - log_sum[i];
         return Choice{ordered((double)score + lp), i, token};
     };
-    for (int l = tid; l < lists; l += kThreads) heads[l] = candidate(l, 0);
+    for (int l = tid; l < lists; l += kThreads) heads[l] = candidate(l, 0, l == tid ? mine : entry(l, 0));
     __syncthreads();
     const int n = min(lists, p.K);
     if (lists <= p.K) {
         if (tid < lists) chosen[tid] = tid;
     } else {
+        // Of many lists only those whose heads reach the K-th largest of the threads' first heads (its upper half) are ranked.
+        uint32_t bound = 0;
+        if (lists > 64) {
+            uint32_t most = 0;
+            for (int l = tid; l < lists; l += kThreads) most = max(most, (uint32_t)(heads[l].score >> 32));
+            tops[tid >> 5][tid & 31] = warp_sort(most, tid & 31);
+            __syncthreads();
+            uint32_t list = tops[0][tid & 31];
+            for (int w = 1; w < kWarps; ++w) list = warp_merge(list, tops[w][tid & 31], tid & 31);
+            bound = __shfl_sync(0xffffffffu, list, p.K - 1);
+        }
         for (int l = tid; l < lists; l += kThreads) {
-            const Choice mine = heads[l];
-            int rank = 0;   // (heads that are none come last, in the order of their lists)
-            for (int j = 0; j < lists; ++j) rank += before(heads[j], mine) || (mine.score == 0 && heads[j].score == 0 && j < l);
+            if ((uint32_t)(heads[l].score >> 32) < bound) continue;
+            const int at = atomicAdd(&n_ranked, 1);
+            ranked[at] = heads[l].score;
+            ranked_list[at] = l;
+        }
+        __syncthreads();
+        for (int e = tid; e < n_ranked; e += kThreads) {
+            const uint64_t score = ranked[e];
+            const int l = ranked_list[e];
+            int rank = 0;   // of equal scores the earlier list has the lower beam, or the lower token
+#pragma unroll 8
+            for (int j = 0; j < n_ranked; ++j) rank += (ranked[j] > score) | ((ranked[j] == score) & (ranked_list[j] < l));
             if (rank < p.K) chosen[rank] = l;
         }
     }
     __syncthreads();
     for (int e = tid; e < n * p.K; e += kThreads) {
         const int l = e / p.K, k = e - l * p.K;
-        lists_of[l][k] = k == 0 ? heads[chosen[l]] : candidate(chosen[l], k);
+        lists_of[l][k] = k == 0 ? heads[chosen[l]] : candidate(chosen[l], k, entry(chosen[l], k));
     }
     __syncthreads();
     if (tid >= 32) return;

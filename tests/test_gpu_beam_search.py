@@ -212,3 +212,13 @@ def test_rows_in_an_order(pkg, cuda, order):
     scores = -torch.arange(I, dtype=F32).expand(B, I).contiguous().to(cuda) / 7
     for K in (1, 4, 32):
         _check(pkg, logits, scores, K)
+
+
+@pytest.mark.parametrize("I,K", [(32, 32), (32, 1), (8, 32), (20, 7)])
+@pytest.mark.parametrize("equal", [False, True])
+def test_rows_that_many_share(pkg, cuda, I, K, equal):
+    """Few rows, each gone over by many: hundreds of lists to choose from, and all of them alike."""
+    logits, scores = _random(cuda, 1, I, 65529, F32, seed=9)
+    if equal:
+        logits, scores = torch.zeros_like(logits), torch.zeros_like(scores)
+    _check(pkg, logits, scores, K)
