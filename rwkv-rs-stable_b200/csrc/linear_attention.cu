@@ -243,37 +243,42 @@ scan_kernel(const ScanArgs args) {
     }
 }
 
-// Four elements a thread; the parts of several segments are on their way at once.
+// Four elements a thread; the parts of several segments are on their way at once, and the first of them while the powers are taken.
 __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args) {
     wait_for_previous();
     const LinearAttentionPass &p = args.p;
     const int64_t quads = p.N * p.N / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, chain = i / quads;
     if (chain >= p.B * p.H) return;
     float4 *at = reinterpret_cast<float4 *>(args.parts) + chain * args.segments * quads + i % quads;
-    const int64_t len = p.lens == nullptr ? p.T : min(max((int64_t)p.lens[chain / p.H], (int64_t)0), p.T);
-    const float lambda = p.log_decay[chain % p.H];
-    float4 s = *at;
     constexpr int kAhead = 8;
-    for (int64_t o = 1; o < args.segments; o += kAhead) {
-        float4 part[kAhead];
+    float4 s = *at, part[kAhead];
+    auto load = [&](int64_t o) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (o + j < args.segments) part[j] = at[(o + j) * quads];
+    };
+    load(1);
+    const int64_t len = p.lens == nullptr ? p.T : min(max((int64_t)p.lens[chain / p.H], (int64_t)0), p.T);
+    const double lambda = (double)p.log_decay[chain % p.H];
+    // d^(tokens of a segment): of a whole one, and of the one that the sequence ends in
+    const float whole = (float)exp(lambda * (double)args.tokens), last = len % args.tokens == 0 ? 1.f : (float)exp(lambda * (double)(len % args.tokens));
+    for (int64_t o = 1; o < args.segments; o += kAhead) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             if (o + j >= args.segments) break;
             // s_o = d^(tokens of the segment before) s_(o-1) + what that adds
             const int64_t from = (p.reversed ? args.segments - (o + j) : o + j - 1) * args.tokens;
-            const int64_t tokens = max((int64_t)0, min(len, from + args.tokens) - from);
-            const float f = tokens == 0 ? 1.f : (float)exp((double)lambda * (double)tokens);
+            const float f = len >= from + args.tokens ? whole : len > from ? last : 1.f;
             s = make_float4(fmaf(s.x, f, part[j].x), fmaf(s.y, f, part[j].y), fmaf(s.z, f, part[j].z), fmaf(s.w, f, part[j].w));
             at[(o + j) * quads] = s;
         }
+        load(o + kAhead);
     }
 }
 
-// CTAs of a pass that an SM holds, by registers and shared memory.
-int64_t places(const LinearAttentionPass &p) { return (int64_t)p.num_sms * (p.N == 128 ? 2 : 8); }
+// CTAs of a pass on an SM, by registers (N = 128: one, and another's worth of segments).  fp32, 1000 tokens: 48 chains of N = 64 backwards 242 us with
+// 8, 217 with 6, 237 with 5; 128 of N = 32 84 us with 8, 72 with 12, 67 with 16; 64 of N = 128 514, 399 and 414 with 1, 2 and 3.
+int64_t places(const LinearAttentionPass &p) { return (int64_t)p.num_sms * (p.N == 128 ? 2 : p.N == 64 ? 6 : 16); }
 
 template <typename T, int N>
 int launch_scan(const ScanArgs &args, cudaStream_t stream) {
