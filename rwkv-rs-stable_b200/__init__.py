@@ -670,11 +670,12 @@ class _LinearAttentionFunction(torch.autograd.Function):
 
 
 def linear_attention_autograd(initial_state: Optional[torch.Tensor], inputs: LinearAttentionForwardInputs):
-    """Differentiable linear attention: ``(output, next_state)`` with gradients to query, key, value and the initial state."""
+    """Differentiable linear attention: ``(output, next_state)`` with gradients to query, key, value and the initial state.
+    A backward pass may be captured into a CUDA graph once no graph that ran eagerly on the same leaves is alive."""
     if inputs.log_decay.requires_grad:
         raise KernelInputsError(8, "Unsupported: linear_attention has no gradient for log_decay; pass it detached")
     return _LinearAttentionFunction.apply(*(t.contiguous() for t in (inputs.query, inputs.key, inputs.value)), inputs.log_decay,
-                                          inputs.context_lens, initial_state)
+                                          inputs.context_lens, None if initial_state is None else initial_state.contiguous())
 
 
 # ------------------------------------------------------------- residual norm --
@@ -754,7 +755,8 @@ class _ResidualNormFunction(torch.autograd.Function):
 
 
 def residual_norm_autograd(inputs: ResidualNormForwardInputs):
-    """Differentiable :func:`residual_norm_custom`: ``(next_residual or None, normed or None)``."""
+    """Differentiable :func:`residual_norm_custom`: ``(next_residual or None, normed or None)``.  Captured as
+    :func:`linear_attention_autograd` is."""
     return _ResidualNormFunction.apply(inputs.kind, inputs.epsilon, *(None if t is None else t.contiguous() for t in inputs.eight()))
 
 

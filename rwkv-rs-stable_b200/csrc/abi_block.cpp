@@ -246,7 +246,6 @@ int check_norm(const NormTensors &t, int32_t kind, double epsilon, ResidualNormA
     p.epsilon = (float)epsilon;
     p.layer = kind == RWKV7_NORM_LAYER;
     p.bf16 = x.t->dtype == RWKV7_BF16;
-    p.device = x.t->device;
     return RWKV7_OK;
 }
 

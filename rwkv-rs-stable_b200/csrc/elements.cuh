@@ -15,20 +15,6 @@ __device__ __forceinline__ float ldf(const __nv_bfloat16 *p) {
 __device__ __forceinline__ void stf(float *p, float x) { *p = x; }
 __device__ __forceinline__ void stf(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-__device__ __forceinline__ void ld8(float (&v)[8], const float *p) {
-    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void unpack8(float (&v)[8], const uint4 &u) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void ld8(float (&v)[8], const __nv_bfloat16 *p) { unpack8(v, *reinterpret_cast<const uint4 *>(p)); }
 __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);

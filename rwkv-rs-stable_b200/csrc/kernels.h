@@ -255,7 +255,7 @@ struct ResidualNormArgs {
     int64_t rows, C;
     bool layer;   // else rms
     bool bf16;
-    int device, num_sms;
+    int num_sms;
 };
 struct ResidualNormBackwardArgs {
     ResidualNormArgs f;                                    // (its outputs are not used)

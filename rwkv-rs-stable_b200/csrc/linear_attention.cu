@@ -16,7 +16,9 @@
 //
 // S is in registers: a thread holds four rows x 16 columns, the columns in groups of four that alternate between the threads of a
 // row, so that these read neighbouring pieces.  A token then costs 64 multiply-adds for nine loads from shared memory; one row a
-// thread needed sixteen for 32.  Bound by the fp32 units for many tokens and by the bytes of S for one.
+// thread needed sixteen for 32.  For one token it is bound by the bytes of S (512 sequences of 40 heads 119 us, 5.7 TB/s); for many by the chain of a
+// block, 5.3 us at N = 64 on two warps, which several CTAs an SM overlap (2 x 1000 tokens of 12 heads in fp32 42 us, three launches of
+// segments of two blocks).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

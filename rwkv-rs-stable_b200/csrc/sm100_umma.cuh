@@ -219,10 +219,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, int x, int 
                  ::"l"(map), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
-// Brings a tile into L2.
-__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *map, int x, int y, int z) {
-    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
-}
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Waits until at most N of the calling thread's bulk groups are still reading their shared-memory source.
 template <int N>

@@ -279,3 +279,51 @@ def test_smaller_workspaces_are_taken(pkg, cuda):
     with pytest.raises(pkg.KernelInputsError) as e:
         _call(pkg, x, workspace=torch.empty(64, dtype=torch.uint8, device=cuda)[8:])
     assert e.value.kind == "Unsupported"
+
+
+@pytest.mark.parametrize("B,T,H", [(40, 17, 5), (40, 47, 5), (40, 48, 5), (1, 32, 148), (1, 47, 149), (1, 513, 40)])
+def test_few_tokens_of_many_chains(pkg, cuda, B, T, H):
+    """On both sides of what decides between the kernels."""
+    _check_forward(pkg, _inputs(cuda, B, T, H, 64, BF16)[0], BF16)
+
+
+@pytest.mark.parametrize("T", [1, 200])
+def test_autograd_captured(pkg, cuda, T):
+    x, dy, ds = _inputs(cuda, 1, T, 3, 64, BF16, seed=1)
+    leaves = [x[n].requires_grad_() for n in ("q", "k", "v", "s0")]
+
+    def step():
+        y, s = pkg.linear_attention_autograd(x["s0"], pkg.LinearAttentionForwardInputs(x["q"], x["k"], x["v"], x["log_decay"]))
+        return torch.autograd.grad((y, s), leaves, (dy, ds))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    new = _inputs(cuda, 1, T, 3, 64, BF16, seed=2)
+    with torch.no_grad():
+        for n in ("q", "k", "v", "s0"):
+            x[n].copy_(new[0][n])
+        dy.copy_(new[1])
+        ds.copy_(new[2])
+    graph.replay()
+    want = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_autograd_of_strided_inputs(pkg, cuda):
+    """Views of a projection of all three and a state out of a larger one: the autograd form lays them out itself."""
+    x, dy, ds = _inputs(cuda, 2, 40, 2, 64, BF16)
+    want = torch.autograd.grad(pkg.linear_attention_autograd(
+        x["s0"], pkg.LinearAttentionForwardInputs(*(x[n].requires_grad_() for n in ("q", "k", "v")), x["log_decay"])),
+        [x[n] for n in ("q", "k", "v")], (dy, ds))
+    qkv = torch.stack([x[n].detach() for n in ("q", "k", "v")], dim=3).requires_grad_()
+    s0 = torch.stack([x["s0"], x["s0"]], dim=-1)[..., 0]
+    out = pkg.linear_attention_autograd(s0, pkg.LinearAttentionForwardInputs(*qkv.unbind(3), x["log_decay"]))
+    got, = torch.autograd.grad(out, qkv, (dy, ds))
+    assert all(torch.equal(a, b) for a, b in zip(got.unbind(3), want))
