@@ -5,6 +5,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <memory>
+#include <new>
 
 #include "abi_common.h"
 #include "check.h"
@@ -442,12 +444,32 @@ int rwkv7_beam_reorder(const rwkv7_tensor *const *states, int32_t n, const rwkv7
             RWKV7_TRY(check_contiguous(o));
         }
     }
+    // What is written stays apart from everything else; states that are only read may be the same.  (Places once a tensor: n (3 n - 1) / 2
+    // pairs are compared.)
+    struct Place {
+        uintptr_t from, to;
+        bool meets(const Place &x) const { return from < x.to && x.from < to; }
+    };
+    auto place = [](const rwkv7_tensor *t) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(t->data);
+        return Place{from, from + bytes_of(t)};
+    };
+    const std::unique_ptr<Place[]> places(new (std::nothrow) Place[2 * (size_t)n]);
+    if (places == nullptr) return fail(RWKV7_ERR_BAD_ARGUMENT, "BadArgument: %d tensors", n);
+    Place *const read = places.get(), *const written = read + n;
     for (int i = 0; i < n; ++i) {
-        // (what is written stays apart from everything else; states that are only read may be the same)
-        const TensorInfo to{out == nullptr ? "states" : "out", out == nullptr ? states[i] : out[i]};
-        RWKV7_TRY(check_apart(to, parents));
-        for (int j = 0; j < i; ++j) RWKV7_TRY(check_apart(to, TensorInfo{to.name, out == nullptr ? states[j] : out[j]}));
-        for (int j = 0; out != nullptr && j < n; ++j) RWKV7_TRY(check_apart(to, TensorInfo{"states", states[j]}));
+        read[i] = place(states[i]);
+        written[i] = out == nullptr ? read[i] : place(out[i]);
+    }
+    const char *name = out == nullptr ? "states" : "out";
+    const Place chosen = place(parents_t);
+    for (int i = 0; i < n; ++i) {
+        const char *met = written[i].meets(chosen) ? "parents" : nullptr;
+        for (int j = 0; j < i && met == nullptr; ++j)
+            if (written[i].meets(written[j])) met = name;
+        for (int j = 0; out != nullptr && j < n && met == nullptr; ++j)
+            if (written[i].meets(read[j])) met = "states";
+        if (met != nullptr) return fail(RWKV7_ERR_BAD_ARGUMENT, "BadArgument: %s and %s share memory", name, met);
     }
     if (I > 32 || (n > 0 && B > 0 && I < 1))
         return fail(RWKV7_ERR_UNSUPPORTED, "Unsupported: beam_reorder from %lld beams (1 to 32)", (long long)I);

@@ -136,35 +136,50 @@ at::Tensor like(const at::Tensor &t) {
     return t.is_contiguous() ? empty(t.sizes(), t.scalar_type(), t) : at::empty_like(t);
 }
 
-// The outputs of a call, each like its own tensor.  Small ones share one allocation (at 512-byte boundaries, as the allocator itself
+// The outputs of a call.  Small ones share one allocation (at 512-byte boundaries, as the allocator itself
 // would place them): an output costs 0.9 us to allocate and wrap, and a decode step around WKV7 has thirteen.  Up to 1 MB
 // in all, because up to there the caching allocator cuts blocks from shared 2 MB segments anyway; larger outputs stay
 // separate, so that holding one of them holds no more memory than its own.  For outputs that a step uses up together: whoever keeps or saves a
 // single one keeps the memory of all of the call's, up to that 1 MB.
+struct Output {
+    at::IntArrayRef sizes;
+    at::ScalarType dtype;
+    int64_t numel() const {
+        int64_t n = 1;
+        for (const int64_t x : sizes) n *= x;
+        return n;
+    }
+};
+// False where they do not share one.
+template <int n>
+bool outputs_together(at::Tensor *out, const Output (&what)[n], const at::Tensor &beside) {
+    constexpr size_t kAlign = 512, kMost = (size_t)1 << 20;
+    size_t at_byte[n], total = 0;
+    if (!beside.is_cuda()) return false;
+    for (int i = 0; i < n; ++i) {
+        if (what[i].numel() <= 0) return false;
+        at_byte[i] = total;
+        total += ((size_t)what[i].numel() * c10::elementSize(what[i].dtype) + kAlign - 1) / kAlign * kAlign;
+    }
+    if (total > kMost) return false;
+    const at::Tensor all = empty({(int64_t)total}, at::kByte, beside);
+    for (int i = 0; i < n; ++i) {
+        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(what[i].dtype));
+        out[i].unsafeGetTensorImpl()->set_storage_offset((int64_t)(at_byte[i] / c10::elementSize(what[i].dtype)));
+        out[i].unsafeGetTensorImpl()->set_sizes_contiguous(what[i].sizes);
+    }
+    return true;
+}
+// Each like its own tensor.
 template <typename... Like>
 void outputs_like(at::Tensor *out, const Like &...tensors) {
     constexpr int n = sizeof...(Like);
     const at::Tensor *ts[n] = {&tensors...};
-    constexpr size_t kAlign = 512, kMost = (size_t)1 << 20;
-    size_t at_byte[n], total = 0;
+    const Output what[n] = {Output{tensors.sizes(), tensors.scalar_type()}...};
     bool together = true;
-    for (int i = 0; i < n; ++i) {
-        const at::Tensor &t = *ts[i];
-        together = together && t.is_cuda() && t.is_contiguous() && t.device() == ts[0]->device() && t.layout() == at::kStrided && t.numel() > 0;
-        at_byte[i] = total;
-        total += ((size_t)t.numel() * (size_t)t.element_size() + kAlign - 1) / kAlign * kAlign;
-    }
-    if (!together || total > kMost) {
-        for (int i = 0; i < n; ++i) out[i] = like(*ts[i]);
-        return;
-    }
-    const at::Tensor all = empty({(int64_t)total}, at::kByte, *ts[0]);
-    for (int i = 0; i < n; ++i) {
-        const at::Tensor &t = *ts[i];
-        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), t.dtype());
-        out[i].unsafeGetTensorImpl()->set_storage_offset((int64_t)(at_byte[i] / (size_t)t.element_size()));
-        out[i].unsafeGetTensorImpl()->set_sizes_contiguous(t.sizes());
-    }
+    for (const at::Tensor *t : ts) together = together && t->is_contiguous() && t->device() == ts[0]->device() && t->layout() == at::kStrided;
+    if (together && outputs_together(out, what, *ts[0])) return;
+    for (int i = 0; i < n; ++i) out[i] = like(*ts[i]);
 }
 
 // Scratch memory of a call: freed when the call has been enqueued, i.e. given back to the allocator's stream order.
@@ -733,7 +748,11 @@ PyObject *beam_select(PyObject *const *a) {
     Desc ld(logits), sd(a[1]), fd(a[3]);
     const int64_t K = integer(a[2]), pad = integer(a[4]), B = logits.dim() > 0 ? logits.size(0) : 0;
     if (K < 0) raise(PyExc_ValueError, "num_beams must not be negative");
-    const at::Tensor out[3] = {empty({B, K}, at::kFloat, logits), empty({B, K}, at::kInt, logits), empty({B, K}, at::kInt, logits)};
+    const int64_t shape[2] = {B, K};
+    const Output what[3] = {{shape, at::kFloat}, {shape, at::kInt}, {shape, at::kInt}};
+    at::Tensor out[3];
+    if (!outputs_together(out, what, logits))
+        for (int i = 0; i < 3; ++i) out[i] = empty(shape, what[i].dtype, logits);
     Desc od[3];
     for (int i = 0; i < 3; ++i) od[i].set(out[i]);
     Workspace ws;
