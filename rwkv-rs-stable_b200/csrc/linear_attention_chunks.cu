@@ -14,6 +14,7 @@
 // shared memory they made 160 us of the 133 below).  One CTA an SM runs all of it as a pipeline:
 //   warps 0-7         P of a chunk, then y          (two threads a row: a TMEM lane and a half of its columns)
 //   warps 8 9 12 13   w C of the chunk behind, transposed and in three parts, put into TMEM when the product of this one has read the last
+//                     (where only what a segment adds is wanted, with 0 1 4 5, which take every other chunk)
 //   warps 16 17       S behind a chunk from its product, one row of S a thread
 //   warp 10           issues the products: P, the sum for S', Y2, Y1
 //   warp 11           loads, four chunks ahead, and stores y from where c was
@@ -59,7 +60,8 @@ enum Bar {   // [stage], [parity of the chunk], or one
     kFreeA = kFull + kStages, kFreeB = kFreeA + kStages,  // the last product that reads it is done
     kYStored = kFreeB + kStages,
     kAddDone = kYStored + kStages, kAddRead = kAddDone + 2,
-    kPDone = kAddRead + 2, kPReady, kYDone, kYRead, kWReady, kSReady, kEnd, kBarCount
+    kWReady = kAddRead + 2,
+    kPDone = kWReady + 2, kPReady, kYDone, kYRead, kSReady, kEnd, kBarCount
 };
 constexpr uint32_t kSlot = kBars + kBarCount * 8;   // TMEM address, then the last chunk in each stage with entries that are not finite
 // [stage][column]: 128 x chunk + 127 - the first such token (reversed: + the last)
@@ -70,6 +72,11 @@ static_assert(kSmem <= 232448, "shared memory of a CTA");
 // columns put it; Y1 between them.  Y2; the sums for S' of even and odd chunks; three parts of w C (lanes 0-63).
 constexpr uint32_t kP = 0, kY1 = 32, kY2 = 128, kW = 320;
 __host__ __device__ constexpr uint32_t t_add(int it) { return 192 + (it & 1) * 64; }
+// (without y there is room for those of two chunks)
+template <bool ADDS>
+__host__ __device__ constexpr uint32_t t_w(int it) {
+    return ADDS && (it & 1) ? kP : kW;
+}
 __host__ __device__ constexpr uint32_t p_operand(int kstep) { return kP + (kstep < 4 ? 0 : 64) + kstep * 8; }
 
 struct Maps {
@@ -139,7 +146,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     if (tid == 0) {
         for (int i = 0; i < kBarCount; ++i)
             mbar_init(bar + i, (i >= kYStored && i < kAddDone) || i == kPReady || i == kYRead ? kGroup
-                               : i == kWReady ? kGroup / 2 : (i >= kAddRead && i < kPDone) || i == kSReady ? kN : i < kFreeA ? (ADDS ? 2 : 3) : 1);
+                               : i >= kWReady && i < kPDone ? kGroup / 2 : (i >= kAddRead && i < kWReady) || i == kSReady ? kN : i < kFreeA ? (ADDS ? 2 : 3) : 1);
         mbar_fence_init();
         for (int i = 0; i < kStages; ++i) bad_chunk[i] = -1;
     }
@@ -236,13 +243,13 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                     umma_commit(bar + kPDone);
                 }
                 // (the sum of two chunks ago has been read: S behind it was published before the last Y2)
-                if (!wait(kWReady, ph) || (ADDS && it >= 2 && !wait_turn(kAddRead, it - 2))) break;
+                if (!wait_turn(kWReady, it) || (ADDS && it >= 2 && !wait_turn(kAddRead, it - 2))) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int part = 0; part < 3; ++part)
 #pragma unroll
                     for (int k = 0; k < kL / 16; ++k)
-                        umma_f16_ts(tmem + t_add(it), tmem + kW + part * 64 + k * 8, make_smem_desc(at + kB + k * 2048, kTile, 1024), id_mn, part > 0 || k > 0);
+                        umma_f16_ts(tmem + t_add(it), tmem + t_w<ADDS>(it) + part * 64 + k * 8, make_smem_desc(at + kB + k * 2048, kTile, 1024), id_mn, part > 0 || k > 0);
                 umma_commit(bar + kAddDone + ph);
                 umma_commit(bar + kFreeB + it % kStages);
                 if (ADDS) continue;
@@ -341,7 +348,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         }
         if (ok && ADDS) write(parts + (size_t)(order + 1) * (kN * kN));
         if (ok && !ADDS && order == p.segments - 1 && p.s_out != nullptr) write(p.s_out + (size_t)chain * (kN * kN));
-    } else if (warp >= 8 && (warp & 2) == 0) {
+    } else if ((ADDS || warp >= 8) && (warp & 2) == 0) {
         // ---- w C, transposed and in three parts: 32 columns of c (TMEM lanes) and 64 tokens a warp, in fragments of 8 x 8: a register holds
         // tokens t and t + 1 of a column, two registers columns eight apart
         const int quarter = warp & 1, token0 = (warp >> 2 & 1) * 64;
@@ -357,7 +364,8 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
             }
         };
         weigh(kL);
-        for (int it = 0; it < count; ++it) {
+        // (without y its warps take the odd chunks)
+        for (int it = ADDS && warp < 8 ? 1 : 0; it < count; it += ADDS ? 2 : 1) {
             const int stage = it % kStages, n = tokens_of(it);
             const uint32_t tile_b = stage * kStage + kB, tile_c = stage * kStage + kC;
             wait_stage(kFull, it);
@@ -404,11 +412,12 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                         lo[i / 4][r] = pack2(sub2(x, unpack2(mid[i / 4][r])));
                     }
                 }
-                if (side == 0 && it > 0) {   // the product that reads the last one's is done
-                    wait_turn(kAddDone, it - 1);
+                constexpr int kBehind = ADDS ? 2 : 1;
+                if (side == 0 && it >= kBehind) {   // the product that reads what is there is done
+                    wait_turn(kAddDone, it - kBehind);
                     tc_fence_after();
                 }
-                const uint32_t at = tmem + kW + t_lane + ((uint32_t)(side * 16) << 16) + token0 / 2;
+                const uint32_t at = tmem + t_w<ADDS>(it) + t_lane + ((uint32_t)(side * 16) << 16) + token0 / 2;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     tmem_st_fragments(at + i * 16, hi[i]);
@@ -419,7 +428,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
             tmem_st_wait();
             fence_proxy_async();
             tc_fence_before();
-            mbar_arrive(bar + kWReady);
+            mbar_arrive(bar + kWReady + (it & 1));
         }
     } else if (!ADDS && warp < 8) {
         // ---- P of a chunk, then y
