@@ -490,32 +490,40 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 tc_fence_before();
                 mbar_arrive(bar + kPReady);
             }
-            wait(kYDone, it & 1);
-            tc_fence_after();
+            // Y2 is there before Y1: it is read, and given its decay, while P C is on its way; once Y1 is read, the next P may be.
             const uint32_t tile_c = it % kStages * kStage + kC;
             const float f = dec[REVERSED ? max(n - 1 - row, 0) : row + 1];
-#pragma unroll 1
+            float2 y[kN / 4];
+            wait_stage(kFreeA, it);
+            tc_fence_after();
+#pragma unroll
             for (int part = 0; part < 2; ++part) {
-                uint32_t v[16], u[16];
-                tmem_ld16(tmem + kY1 + t_lane + c0 + part * 16, v);
+                uint32_t u[16];
                 tmem_ld16(tmem + kY2 + t_lane + c0 + part * 16, u);
                 tmem_ld_wait();
-                if (part == 1) {
-                    tc_fence_before();
-                    mbar_arrive(bar + kYRead);
-                }
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), make_float2(f, f),
-                                                make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                    u[e / 2] = pack2(x);
-                }
-                if (row >= n) {
+                for (int e = 0; e < 8; ++e)
+                    y[part * 8 + e] = __fmul2_rn(make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])), make_float2(f, f));
+            }
+            wait(kYDone, it & 1);
+            tc_fence_after();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) u[e] = 0u;
-                }
-                sts16(base + tile_c + piece(row, half * 4 + 2 * part), make_uint4(u[0], u[1], u[2], u[3]));
-                sts16(base + tile_c + piece(row, half * 4 + 2 * part + 1), make_uint4(u[4], u[5], u[6], u[7]));
+            for (int part = 0; part < 2; ++part) {
+                uint32_t v[16];
+                tmem_ld16(tmem + kY1 + t_lane + c0 + part * 16, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    y[part * 8 + e] = __fadd2_rn(y[part * 8 + e], make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])));
+            }
+            tc_fence_before();
+            mbar_arrive(bar + kYRead);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = row < n ? pack2(y[q * 4 + e]) : 0u;
+                sts16(base + tile_c + piece(row, half * 4 + q), make_uint4(u[0], u[1], u[2], u[3]));
             }
             if (bad_chunk[it % kStages] == it && row < n) put_nan(smem + tile_c, row, half, bad_from + it % kStages * kN, it * kL, REVERSED);
             fence_proxy_async();
