@@ -11,14 +11,14 @@
 // Four products of a chunk: P = A B^T [128 x 128], Y2 = A S [128 x 64], the sum for S' = (w C)^T B [64 x 64] and, once P carries
 // its decays and its mask, Y1 = P C [128 x 64].  HBM gives an SM a chunk's 64 KB in 1.5 us.  What is scarcer is shared memory's
 // 128 bytes a cycle, which the products' operands, the loads and everything else share: so P and w C are operands in TMEM (as operands in
-// shared memory they made 160 us of the 133 below).  One CTA an SM runs all of it as a pipeline:
+// shared memory they made 160 us of the 129 below).  One CTA an SM runs all of it as a pipeline:
 //   warps 0-7         P of a chunk, then y          (two threads a row: a TMEM lane and a half of its columns)
 //   warps 8 9 12 13   w C of the chunk behind, transposed and in three parts, put into TMEM when the product of this one has read the last
 //                     (where only what a segment adds is wanted, with 0 1 4 5, which take every other chunk)
 //   warps 16 17       S behind a chunk from its product, one row of S a thread
 //   warp 10           issues the products: P, the sum for S', Y2, Y1
 //   warp 11           loads, four chunks ahead, and stores y from where c was
-// 8 x 4096 tokens of 32 heads: 133 us, 4.1 TB/s, 2.4 us a chunk and SM.  What bounds it is the chain of a chunk through the roles: its state waits
+// 8 x 4096 tokens of 32 heads: 129 us, 4.2 TB/s, 2.3 us a chunk and SM.  What bounds it is the chain of a chunk through the roles: its state waits
 // for its sum, its sum for w C, y for P's decays, and each of these hands over through a barrier.
 //
 // Precision: y is rounded to bf16, and so is P (once); S stays in fp32 registers and enters Y2 as hi + lo (16 bits and a
@@ -231,7 +231,8 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         if (elect_one()) {
             constexpr uint32_t id_p = make_idesc(kFmtBF16, 128, 128, false, false), id_y2 = make_idesc(kFmtBF16, 128, 64, false, false),
                                id_mn = make_idesc(kFmtBF16, 128, 64, false, true);
-            // P first, for what waits for it takes longest; while it is given its decays, the sum for S' and Y2 follow.
+            // P first, for what waits for it takes longest; while it is given its decays, the sum for S' and Y2 follow.  (A third of the sum in
+            // front of P made 135 us of 129, Y2 in front of the sum 144.)
             for (int it = 0; it < count; ++it) {
                 const uint32_t at = base + it % kStages * kStage, ph = it & 1;
                 if (!ADDS) {
