@@ -16,8 +16,8 @@
 //
 // S is in registers: a thread holds four rows x 16 columns, the columns in groups of four that alternate between the threads of a
 // row, so that these read neighbouring pieces.  A token then costs 64 multiply-adds for nine loads from shared memory; one row a
-// thread needed sixteen for 32.  For one token it is bound by the bytes of S (512 sequences of 40 heads 119 us, 5.7 TB/s); for many by the chain of a
-// block, 5.3 us at N = 64 on two warps, which several CTAs an SM overlap (2 x 1000 tokens of 12 heads in fp32 42 us, three launches of
+// thread needed sixteen for 32.  For one token it is bound by the bytes of S (512 sequences of 40 heads 112 us, 6.1 TB/s); for many by the chain of a
+// block, 5.3 us at N = 64 on two warps, which several CTAs an SM overlap (2 x 1000 tokens of 12 heads in fp32 43 us, three launches of
 // segments of two blocks).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -39,6 +39,9 @@ struct Shape {
     static constexpr int kShare = N / kCols;                       // threads of a row
     static constexpr int kThreads = N / kRows * kShare;
     static constexpr int kPitch = N + 4;                           // floats of a staged row
+    // CTAs an SM is to hold, which spills a few of 160 registers: one token of 512 sequences of 40 heads 118 -> 112 us, 4 x 1000 fp32 tokens of 32
+    // heads 177 -> 157, N = 128 of 16 heads 397 -> 308.  The pass that only adds to states spills more than it gains at N = 64.
+    static constexpr int resident(bool adds) { return N == 128 ? 2 : N == 64 ? (adds ? 1 : 8) : 16; }
 };
 
 struct ScanArgs {
@@ -65,7 +68,7 @@ __device__ __forceinline__ void scatter_sums(float (&v)[SHARE][ROWS], int part) 
 
 // ADDS: only what a segment adds to the state.
 template <typename T, int N, bool REVERSED, bool ADDS>
-__global__ void __launch_bounds__(Shape<N>::kThreads)
+__global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::resident(ADDS))
 scan_kernel(const ScanArgs args) {
     using Sh = Shape<N>;
     constexpr int R = Sh::kRows, SHARE = Sh::kShare, THREADS = Sh::kThreads, PITCH = Sh::kPitch;
@@ -278,9 +281,9 @@ __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args
     }
 }
 
-// CTAs of a pass on an SM, by registers (N = 128: one, and another's worth of segments).  fp32, 1000 tokens: 48 chains of N = 64 backwards 242 us with
-// 8, 217 with 6, 237 with 5; 128 of N = 32 84 us with 8, 72 with 12, 67 with 16; 64 of N = 128 514, 399 and 414 with 1, 2 and 3.
-int64_t places(const LinearAttentionPass &p) { return (int64_t)p.num_sms * (p.N == 128 ? 2 : p.N == 64 ? 6 : 16); }
+// CTAs of a pass on the device: segments fill them.  fp32: 4 x 1000 tokens of 32 heads at N = 64 184 us with 6 an SM, 170 with 7, 157 with 8; 84, 72 and 67
+// at N = 32 with 8, 12 and 16; 64 chains of 1000 at N = 128 514, 399 and 414 with 1, 2 and 3.
+int64_t places(const LinearAttentionPass &p) { return (int64_t)p.num_sms * (p.N == 128 ? 2 : p.N == 64 ? 8 : 16); }
 
 template <typename T, int N>
 int launch_scan(const ScanArgs &args, cudaStream_t stream) {
