@@ -355,13 +355,15 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         const int quarter = warp & 1, token0 = (warp >> 2 & 1) * 64;
         const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
         const int q = lane & 3;
-        // the weights of this lane's pairs of tokens, token0 + 8 i + 2 q and the next, of a chunk of n
+        // the weights of this lane's pairs of tokens, token0 + 8 i + 2 q and the next, of a chunk of n; behind the sequence, where c is zero, powers
+        // that are part of nothing may be infinite and are not taken (d^0 instead)
         float2 w[8];
+        int weighed = kL;
         auto weigh = [&](int n) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int t = token0 + 8 * i + 2 * q;   // (behind the sequence c is zero)
-                w[i] = make_float2(dec[REVERSED ? t + 1 : max(n - 1 - t, 0)], dec[REVERSED ? t + 2 : max(n - 2 - t, 0)]);
+                const int t = token0 + 8 * i + 2 * q;
+                w[i] = make_float2(dec[!REVERSED ? max(n - 1 - t, 0) : t < n ? t + 1 : 0], dec[!REVERSED ? max(n - 2 - t, 0) : t + 1 < n ? t + 2 : 0]);
             }
         };
         weigh(kL);
@@ -380,7 +382,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 }
                 __syncwarp();
             }
-            if (!REVERSED && (n < kL || (it > 0 && tokens_of(it - 1) < kL))) weigh(n);
+            if (n != weighed) weigh(weighed = n);   // (reversed the sequence's last chunk is the first)
 #pragma unroll 1
             for (int side = 0; side < 2; ++side) {   // sixteen columns (lanes) at a time
                 // sixteen tokens: matrices (tokens, columns), (tokens, columns + 8), (tokens + 8, ..), (tokens + 8, .. + 8)

@@ -1,0 +1,34 @@
+"""Linear attention on values at the edges: decays above one, long memories, infinities, and how many bits of a state are kept.
+
+Bounds are those of ``block_reference``, or are derived at the test."""
+import pytest
+import torch
+
+import block_reference as ref
+from test_gpu_linear_attention import BF16, F32, _abs, _call, _close, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,lens", [(100, None), (300, [100, 57]), (3000, [100, 0])])
+def test_states_that_double_every_token(pkg, cuda, T, lens, dtype):
+    """exp(0.7 x 100) is a number, exp(0.7 x 128) is not: powers behind a sequence's end are part of nothing, in either direction, in
+    one piece or in segments."""
+    B = 1 if lens is None else len(lens)
+    x, dy, ds = _inputs(cuda, B, T, 2, 64, dtype, seed=T, lens=lens)
+    x["log_decay"] = torch.tensor([0.7, 0.35], device=cuda)
+    out = _call(pkg, x)
+    inputs = pkg.LinearAttentionForwardInputs(x["q"], x["k"], x["v"], x["log_decay"], context_lens=x["lens"])
+    grads, ds0 = pkg.linear_attention_backward(inputs, dy, ds, initial_state=x["s0"])
+    live = T if lens is None else max(lens)   # (the 64-bit form takes powers of every place)
+    y = {n: t[:, :live] if n in ("q", "k", "v") else t for n, t in x.items()}
+    inside = torch.arange(live, device=cuda) < (torch.full((B,), T, device=cuda) if lens is None else x["lens"])[:, None]
+    dy0 = torch.where(inside[:, :, None, None], dy[:, :live], torch.zeros_like(dy[:, :live]))
+    wants = [*ref.attention(**y), *ref.attention_grads(**y, dy=dy0, ds=ds)]
+    mags = [*ref.attention(**_abs(y)), *ref.attention_grads(**_abs(y), dy=dy0.abs(), ds=ds.abs())]
+    for name, got, w, m in zip(("output", "state", "query", "key", "value", "state gradient"), (out.output, out.next_state, *grads, ds0), wants, mags):
+        if got.dim() == 4 and got.shape[1] == T and name not in ("state", "state gradient"):
+            assert bool((got[:, live:] == 0).all()), name
+            got = got[:, :live]
+        _close(got, w, m, live, 64, dtype, name)
