@@ -536,9 +536,9 @@ int rwkv7_lm_head_ce_finalize(const rwkv7_tensor *partials_all, const rwkv7_tens
  * Per (b,h), d = exp(log_decay[h]), S[i][j] (i value row, j key column), t = 0 .. len_b - 1:
  *   S[i][j] = d S[i][j] + value[b,t,h,i] key[b,t,h,j];   output[b,t,h,i] = sum_j S[i][j] query[b,t,h,j].
  * query, key, value and output are [B,T,H,N], all F32 or all BF16, N = 32, 64 or 128; T >= 1.  log_decay is [H] F32 (a model
- * has values up to 0; larger ones are computed as the formula says while exp(len_b log_decay) is a finite fp32 number, and may give
- * NaN beyond), states are [B,H,N,N] F32; sums and the carried state are fp32.  initial_state may be NULL (zero) and next_state NULL (not wanted); they may be the same tensor.  No scale is applied
- * to the queries.
+ * has values up to 0; larger ones are computed as the formula says while exp(len_b log_decay) is a finite fp32 number; beyond that
+ * results are not defined), states are [B,H,N,N] F32; sums and the carried state are fp32.  initial_state may be NULL (zero) and
+ * next_state NULL (not wanted); they may be the same tensor.  No scale is applied to the queries.
  * context_lens ([B] I32, may be NULL) gives each sequence of a padded batch its length, 0 .. T (smaller values count as 0, larger
  * ones as T): the tokens behind it are not read into anything, their output is zero, and the final state is the one at the length.
  * The workspace lets a call of few chains work on several parts of a sequence at once; a smaller one than the call below names, or

@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cfloat>
 #include <mutex>
 
 #include "elements.cuh"
@@ -164,7 +165,8 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     if (warp != kMmaWarp && warp != kLoadWarp) {
         const float lambda = p.log_decay[h];
         auto power = [&](int k) { return k == 0 ? 1.f : expf(lambda * (float)k); };   // d^k; d^0 is 1 for every d
-        if (tid <= kL) dec[tid] = power(tid);
+        // (reversed, a chunk of fewer than 128 tokens meets powers behind its last one times zero: where d is above one they are kept finite)
+        if (tid <= kL) dec[tid] = REVERSED && power(tid) > FLT_MAX ? FLT_MAX : power(tid);
         const int other = (tid < kMmaWarp * 32 ? tid : tid - 64) - (kL + 1);   // threads that have no entry of dec
         if (other >= 0 && other < 32) col[other] = power(REVERSED ? other : 31 - other);
         // diag[shift][k + shift] for k = e - lane + 31: d^(lane - e) where e <= lane (reversed: d^(e - lane) where e >= lane), else 0
@@ -355,22 +357,22 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         const int quarter = warp & 1, token0 = (warp >> 2 & 1) * 64;
         const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
         const int q = lane & 3;
-        // the weights of this lane's pairs of tokens, token0 + 8 i + 2 q and the next, of a chunk of n; behind the sequence, where c is zero, powers
-        // that are part of nothing may be infinite and are not taken (d^0 instead)
+        // the weights of this lane's pairs of tokens, token0 + 8 i + 2 q and the next, of a chunk of n
         float2 w[8];
-        int weighed = kL;
         auto weigh = [&](int n) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int t = token0 + 8 * i + 2 * q;
-                w[i] = make_float2(dec[!REVERSED ? max(n - 1 - t, 0) : t < n ? t + 1 : 0], dec[!REVERSED ? max(n - 2 - t, 0) : t + 1 < n ? t + 2 : 0]);
+                const int t = token0 + 8 * i + 2 * q;   // (behind the sequence c is zero)
+                w[i] = make_float2(dec[REVERSED ? t + 1 : max(n - 1 - t, 0)], dec[REVERSED ? t + 2 : max(n - 2 - t, 0)]);
             }
         };
-        weigh(kL);
+        int weighed = 0;
+        if (REVERSED) weigh(kL);
         // (without y its warps take the odd chunks)
         for (int it = ADDS && warp < 8 ? 1 : 0; it < count; it += ADDS ? 2 : 1) {
             const int stage = it % kStages, n = tokens_of(it);
             const uint32_t tile_b = stage * kStage + kB, tile_c = stage * kStage + kC;
+            if (!REVERSED && n != weighed) weigh(weighed = n);
             wait_stage(kFull, it);
             if (n < kL) {   // (uniform) behind the sequence anything may stand
 #pragma unroll 1
@@ -382,7 +384,6 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 }
                 __syncwarp();
             }
-            if (n != weighed) weigh(weighed = n);   // (reversed the sequence's last chunk is the first)
 #pragma unroll 1
             for (int side = 0; side < 2; ++side) {   // sixteen columns (lanes) at a time
                 // sixteen tokens: matrices (tokens, columns), (tokens, columns + 8), (tokens + 8, ..), (tokens + 8, .. + 8)
