@@ -25,6 +25,7 @@
 #include "elements.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "linear_attention_decay.cuh"
 #include "linear_attention_plan.h"
 
 namespace rwkv7 {
@@ -266,14 +267,15 @@ __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args
     const int64_t len = p.lens == nullptr ? p.T : min(max((int64_t)p.lens[chain / p.H], (int64_t)0), p.T);
     const double lambda = (double)p.log_decay[chain % p.H];
     // d^(tokens of a segment): of a whole one, and of the one that the sequence ends in
-    const float whole = (float)exp(lambda * (double)args.tokens), last = len % args.tokens == 0 ? 1.f : (float)exp(lambda * (double)(len % args.tokens));
+    SteadyPower whole(exp(lambda * (double)args.tokens));
+    const float last = len % args.tokens == 0 ? 1.f : (float)exp(lambda * (double)(len % args.tokens));
     for (int64_t o = 1; o < args.segments; o += kAhead) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             if (o + j >= args.segments) break;
             // s_o = d^(tokens of the segment before) s_(o-1) + what that adds
             const int64_t from = (p.reversed ? args.segments - (o + j) : o + j - 1) * args.tokens;
-            const float f = len >= from + args.tokens ? whole : len > from ? last : 1.f;
+            const float f = len >= from + args.tokens ? whole.next() : len > from ? last : 1.f;
             s = make_float4(fmaf(s.x, f, part[j].x), fmaf(s.y, f, part[j].y), fmaf(s.z, f, part[j].z), fmaf(s.w, f, part[j].w));
             at[(o + j) * quads] = s;
         }

@@ -16,6 +16,7 @@
 //   warps 8 9 12 13   w C of the chunk behind, transposed and in three parts, put into TMEM when the product of this one has read the last
 //                     (where only what a segment adds is wanted, with 0 1 4 5, which take every other chunk)
 //   warps 16 17       S behind a chunk from its product, one row of S a thread
+//   warp 14           d^128 in 64 bits, for these (its some 0.3 us of code would else stand in front of the first chunk)
 //   warp 10           issues the products: P, the sum for S', Y2, Y1
 //   warp 11           loads, four chunks ahead, and stores y from where c was
 // 8 x 4096 tokens of 32 heads: 129 us, 4.2 TB/s, 2.3 us a chunk and SM.  What bounds it is the chain of a chunk through the roles: its state waits
@@ -37,6 +38,7 @@
 #include "elements.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "linear_attention_decay.cuh"
 #include "linear_attention_plan.h"
 #include "sm100_mma.cuh"
 #include "sm100_umma.cuh"
@@ -55,7 +57,9 @@ constexpr uint32_t kCol = kS + 2 * kSPart;     // d^31 .. d^0 forwards, d^0 .. d
 constexpr uint32_t kDiag = kCol + 128;         // the same continued by zeros (reversed: behind zeros), four times, each a word further on
 constexpr uint32_t kDiagWords = 68;
 constexpr uint32_t kDec = kDiag + 4 * kDiagWords * 4;   // d^0 .. d^128
-constexpr uint32_t kBars = kDec + 520;
+constexpr uint32_t kWhole = kDec + 520;                 // d^128 as the factor of whole chunks
+constexpr uint32_t kBars = kWhole + sizeof(SteadyPower);
+static_assert(sizeof(SteadyPower) == 16 && kBars % 8 == 0);
 enum Bar {   // [stage], [parity of the chunk], or one
     kFull,                                                // a, b and c are loaded
     kFreeA = kFull + kStages, kFreeB = kFreeA + kStages,  // the last product that reads it is done
@@ -143,7 +147,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     volatile int *bad_chunk = reinterpret_cast<volatile int *>(smem + kSlot + 4);
     int *bad_from = reinterpret_cast<int *>(smem + kBad);
     float *dec = reinterpret_cast<float *>(smem + kDec), *col = reinterpret_cast<float *>(smem + kCol), *diag = reinterpret_cast<float *>(smem + kDiag);
-    constexpr int kMmaWarp = 10, kLoadWarp = 11, kStateWarp = 16;   // (w C and S are on lanes 0-63: their warps are numbers 0 and 1 of four)
+    constexpr int kMmaWarp = 10, kLoadWarp = 11, kPowerWarp = 14, kStateWarp = 16;   // (w C and S are on lanes 0-63: their warps are numbers 0 and 1 of four)
     if (tid == 0) {
         for (int i = 0; i < kBarCount; ++i)
             mbar_init(bar + i, (i >= kYStored && i < kAddDone) || i == kPReady || i == kYRead ? kGroup
@@ -328,14 +332,19 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
             fence_proxy_async();
             mbar_arrive(bar + kSReady);
         };
+        SteadyPower whole;
         for (int it = 0; it < count; ++it) {
             if (!ADDS) {
                 if (it > 0) wait_stage(kFreeA, it - 1);   // the Y2 that reads the last one is done
                 publish();
             }
+            if (live >= kL && it == (REVERSED && live % kL != 0 ? 1 : 0)) {   // the first whole chunk
+                asm volatile("bar.sync 2, 96;" ::: "memory");
+                whole = *reinterpret_cast<const SteadyPower *>(smem + kWhole);
+            }
             wait_turn(kAddDone, it);
             tc_fence_after();
-            float dn = dec[tokens_of(it)];
+            float dn = tokens_of(it) == kL ? whole.next() : dec[tokens_of(it)];
             if (bad_chunk[it % kStages] == it && bad_from[it % kStages * kN + row] >= it * kL) dn = __uint_as_float(0x7fffffffu);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -351,6 +360,12 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
         }
         if (ok && ADDS) write(parts + (size_t)(order + 1) * (kN * kN));
         if (ok && !ADDS && order == p.segments - 1 && p.s_out != nullptr) write(p.s_out + (size_t)chain * (kN * kN));
+    } else if (warp == kPowerWarp) {
+        if (live >= kL) {   // (there is a whole chunk: the warps of the state wait for this in front of its sum)
+            if (lane == 0) *reinterpret_cast<SteadyPower *>(smem + kWhole) = SteadyPower(exp((double)p.log_decay[h] * kL));
+            __syncwarp();
+            asm volatile("bar.arrive 2, 96;" ::: "memory");
+        }
     } else if ((ADDS || warp >= 8) && (warp & 2) == 0) {
         // ---- w C, transposed and in three parts: 32 columns of c (TMEM lanes) and 64 tokens a warp, in fragments of 8 x 8: a register holds
         // tokens t and t + 1 of a column, two registers columns eight apart

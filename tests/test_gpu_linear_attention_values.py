@@ -32,3 +32,19 @@ def test_states_that_double_every_token(pkg, cuda, T, lens, dtype):
             assert bool((got[:, live:] == 0).all()), name
             got = got[:, :live]
         _close(got, w, m, live, 64, dtype, name)
+
+
+@pytest.mark.parametrize("dtype,pieces,scalings", [(BF16, "one", 256), (BF16, "segments", 18 + 15), (F32, "one", 2048), (F32, "segments", 148 + 14)])
+def test_a_long_memory_does_not_drift(pkg, cuda, dtype, pieces, scalings):
+    """Without values the state is S0 d^T.  Each of the chunks, blocks or segments that it is scaled over rounds an entry, by half a step at
+    most and this way or that, so that a head's norm is off by the root of their number times a half step; the powers by which it is scaled
+    are off together by a step or two, however many they are."""
+    T, H = 32768, 8
+    x = _inputs(cuda, 1, T, H, 64, dtype, seed=4)[0]
+    x["v"].zero_()
+    x["log_decay"] = -1.3e-5 * torch.arange(1, H + 1, device=cuda, dtype=F32)
+    workspace = torch.empty(0, dtype=torch.uint8, device=cuda) if pieces == "one" else None
+    got = _call(pkg, x, workspace=workspace).next_state.double()
+    want = x["s0"].double() * torch.exp(x["log_decay"].double() * T)[:, None, None]
+    off = ((got - want).flatten(2).norm(dim=2) / want.flatten(2).norm(dim=2)).flatten() / ref.U
+    assert bool((off <= 2 + scalings ** 0.5).all()), off.tolist()
