@@ -338,7 +338,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 if (it > 0) wait_stage(kFreeA, it - 1);   // the Y2 that reads the last one is done
                 publish();
             }
-            if (live >= kL && it == (REVERSED && live % kL != 0 ? 1 : 0)) {   // the first whole chunk
+            if (it == 0 && live >= kL) {
                 asm volatile("bar.sync 2, 96;" ::: "memory");
                 whole = *reinterpret_cast<const SteadyPower *>(smem + kWhole);
             }

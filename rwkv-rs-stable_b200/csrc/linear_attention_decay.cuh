@@ -18,7 +18,7 @@ class SteadyPower {
         down_ = __double2float_rd(power);
         up_ = __double2float_ru(power);
         if (up_ == INFINITY) down_ = INFINITY;   // (nothing to choose from)
-        else if (up_ > down_) up_part_ = (float)((power - (double)down_) / ((double)up_ - (double)down_));
+        else if (up_ > down_) up_part_ = (float)(power - (double)down_) / (up_ - down_);
     }
     __device__ __forceinline__ float next() {
         at_ += up_part_;
