@@ -62,9 +62,9 @@ constexpr uint32_t kBars = kWhole + sizeof(SteadyPower);
 static_assert(sizeof(SteadyPower) == 16 && kBars % 8 == 0);
 enum Bar {   // [stage], [parity of the chunk], or one
     kFull,                                                // a, b and c are loaded
-    kFreeA = kFull + kStages, kFreeB = kFreeA + kStages,  // the last product that reads it is done
+    kFreeA = kFull + kStages, kFreeB = kFreeA + kStages,  // the last product that reads it is done (without y: and S behind the chunk is known)
     kYStored = kFreeB + kStages,
-    kAddDone = kYStored + kStages, kAddRead = kAddDone + 2,
+    kAddDone = kYStored + kStages, kAddRead = kAddDone + 2,   // (the latter without y; with it kSReady says so)
     kWReady = kAddRead + 2,
     kPDone = kWReady + 2, kPReady, kYDone, kYRead, kSReady, kEnd, kBarCount
 };
@@ -151,7 +151,8 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
     if (tid == 0) {
         for (int i = 0; i < kBarCount; ++i)
             mbar_init(bar + i, (i >= kYStored && i < kAddDone) || i == kPReady || i == kYRead ? kGroup
-                               : i >= kWReady && i < kPDone ? kGroup / 2 : (i >= kAddRead && i < kWReady) || i == kSReady ? kN : i < kFreeA ? (ADDS ? 2 : 3) : 1);
+                               : i >= kWReady && i < kPDone ? kGroup / 2 : (i >= kAddRead && i < kWReady) || i == kSReady ? kN
+                               : i < kFreeA ? (ADDS ? 2 : 3) : ADDS && i >= kFreeB && i < kYStored ? 1 + kN : 1);
         mbar_fence_init();
         for (int i = 0; i < kStages; ++i) bad_chunk[i] = -1;
     }
@@ -355,8 +356,11 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                 for (int e = 0; e < 8; ++e)
                     S[q * 8 + e] = __ffma2_rn(S[q * 8 + e], make_float2(dn, dn), make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])));
             }
-            tc_fence_before();
-            mbar_arrive(bar + kAddRead + (it & 1));
+            tc_fence_before();   // (the sum has been read: here for publish's arrival as well)
+            if (ADDS) {          // and the note of what is not finite: both places may be written again
+                mbar_arrive(bar + kAddRead + (it & 1));
+                mbar_arrive(bar + kFreeB + it % kStages);
+            }
         }
         if (ok && ADDS) write(parts + (size_t)(order + 1) * (kN * kN));
         if (ok && !ADDS && order == p.segments - 1 && p.s_out != nullptr) write(p.s_out + (size_t)chain * (kN * kN));

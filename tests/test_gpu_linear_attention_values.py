@@ -48,3 +48,22 @@ def test_a_long_memory_does_not_drift(pkg, cuda, dtype, pieces, scalings):
     want = x["s0"].double() * torch.exp(x["log_decay"].double() * T)[:, None, None]
     off = ((got - want).flatten(2).norm(dim=2) / want.flatten(2).norm(dim=2)).flatten() / ref.U
     assert bool((off <= 2 + scalings ** 0.5).all()), off.tolist()
+
+
+@pytest.mark.parametrize("dtype,T", [(BF16, 148 * 16 * 128 - 77), (F32, 148 * 8 * 16 * 2 - 5)])
+def test_every_entry_that_is_not_finite_is_found_in_segments(pkg, cuda, dtype, T):
+    """One column of the values in each of 64 chunks in a row, so that a column's later tokens and its row of the state hang on
+    a single entry of one segment, with entries of other columns in the chunks around it."""
+    step = 128 if dtype == BF16 else 16
+    x = _inputs(cuda, 1, T, 1, 64, dtype, seed=8)[0]
+    x["log_decay"] = torch.tensor([-0.01], device=cuda)
+    first = torch.tensor([T // 3 // step * step + step * c + 11 * c % step for c in range(64)], device=cuda)
+    for c, t in enumerate(first.tolist()):
+        x["v"][0, t, 0, (29 * c) % 64] = (float("inf"), float("-inf"), float("nan"))[c % 3]
+    got = _call(pkg, x)
+    assert pkg.read_device_status(0) == 0
+    of_column = torch.empty_like(first)
+    of_column[(29 * torch.arange(64, device=cuda)) % 64] = first
+    reached = torch.arange(T, device=cuda)[:, None] >= of_column
+    assert torch.equal(torch.isfinite(got.output[0, :, 0].float()), ~reached)
+    assert not bool(torch.isfinite(got.next_state).any())
