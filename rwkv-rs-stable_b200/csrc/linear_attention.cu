@@ -75,6 +75,8 @@ scan_kernel(const ScanArgs args) {
     constexpr int R = Sh::kRows, SHARE = Sh::kShare, THREADS = Sh::kThreads, PITCH = Sh::kPitch;
     __shared__ __align__(16) float sa[ADDS ? 1 : kBlock * PITCH], sb[kBlock * PITCH], sc[kBlock * PITCH], sp[ADDS ? 1 : kBlock * kBlock];
     __shared__ float dec[kBlock + 1];
+    __shared__ SteadyPower whole;   // d^16, by which S may be scaled again and again
+    __shared__ float scale;         // of the block at hand
     const LinearAttentionPass &p = args.p;
     const int64_t chains = p.B * p.H, chain = blockIdx.x % chains, order = blockIdx.x / chains;
     const int64_t bi = chain / p.H, h = chain % p.H;
@@ -126,14 +128,14 @@ scan_kernel(const ScanArgs args) {
     const int64_t len = p.lens == nullptr ? p.T : min(max((int64_t)p.lens[bi], (int64_t)0), p.T);
     const int64_t seg = REVERSED ? args.segments - 1 - order : order;
     const int64_t begin = min(p.T, seg * args.tokens), end = min(p.T, begin + args.tokens), stop = max(begin, min(len, end));   // live: [begin, stop)
-    // d^k in 64 bits, rounded once; d^0 is 1 for every d.  Of d^16, by which S is scaled again and again, also what the rounding took.
+    // d^k in 64 bits, rounded once; d^0 is 1 for every d.
     const double lambda = (double)p.log_decay[h];
     const int full = stop - begin < kBlock ? (int)(stop - begin) : kBlock;
-    for (int k = tid; k <= full; k += THREADS) dec[k] = k == 0 ? 1.f : (float)exp(lambda * k);
-    float rest = 0.f;
-    if (stop - begin > kBlock) {
-        const double whole = exp(lambda * kBlock);
-        rest = whole < 3.0e38 ? (float)(whole - (double)(float)whole) : 0.f;
+    static_assert(THREADS > kBlock + 1);
+    if (tid <= full || tid == kBlock + 1) {
+        const double power = exp(lambda * min(tid, kBlock));
+        if (tid <= full) dec[tid] = tid == 0 ? 1.f : (float)power;
+        else whole = SteadyPower(power);
     }
     const int64_t step = p.H * N, base = (bi * p.T * p.H + h) * N;   // of token 0
     const T *a = static_cast<const T *>(p.a) + base, *b = static_cast<const T *>(p.b) + base, *c = static_cast<const T *>(p.c) + base;
@@ -144,6 +146,7 @@ scan_kernel(const ScanArgs args) {
         const int64_t first = REVERSED ? begin + (stop - 1 - done) / kBlock * kBlock : done;
         const int n = (int)min((int64_t)kBlock, stop - first);
         __syncthreads();
+        if (tid == 0) scale = n == kBlock ? whole.factor((uint32_t)((done - begin) / kBlock)) : dec[n];
         for (int i = tid; i < n * (N / 4); i += THREADS) {
             const int t = i / (N / 4), j = i % (N / 4) * 4;
             const int64_t at = (first + t) * step + j;
@@ -215,11 +218,11 @@ scan_kernel(const ScanArgs args) {
             }
         }
         // S' (the last block's is not needed where nobody takes it)
-        const float dn = dec[n], dl = n == kBlock ? rest : 0.f;
+        const float dn = scale;
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int m = 0; m < 8; ++m) S[r][m] = __ffma2_rn(S[r][m], make_float2(dn, dn), __fmul2_rn(S[r][m], make_float2(dl, dl)));
+            for (int m = 0; m < 8; ++m) S[r][m] = __fmul2_rn(S[r][m], make_float2(dn, dn));
 #pragma unroll 2
         for (int j = 0; j < n; ++j) {
             const float w = dec[REVERSED ? j + 1 : n - 1 - j];
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args
     const int64_t len = p.lens == nullptr ? p.T : min(max((int64_t)p.lens[chain / p.H], (int64_t)0), p.T);
     const double lambda = (double)p.log_decay[chain % p.H];
     // d^(tokens of a segment): of a whole one, and of the one that the sequence ends in
-    SteadyPower whole(exp(lambda * (double)args.tokens));
+    const SteadyPower whole(exp(lambda * (double)args.tokens));
     const float last = len % args.tokens == 0 ? 1.f : (float)exp(lambda * (double)(len % args.tokens));
     for (int64_t o = 1; o < args.segments; o += kAhead) {
 #pragma unroll
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(256) segment_states_kernel(const ScanArgs args
             if (o + j >= args.segments) break;
             // s_o = d^(tokens of the segment before) s_(o-1) + what that adds
             const int64_t from = (p.reversed ? args.segments - (o + j) : o + j - 1) * args.tokens;
-            const float f = len >= from + args.tokens ? whole.next() : len > from ? last : 1.f;
+            const float f = len >= from + args.tokens ? whole.factor((uint32_t)(o + j)) : len > from ? last : 1.f;
             s = make_float4(fmaf(s.x, f, part[j].x), fmaf(s.y, f, part[j].y), fmaf(s.z, f, part[j].z), fmaf(s.w, f, part[j].w));
             at[(o + j) * quads] = s;
         }

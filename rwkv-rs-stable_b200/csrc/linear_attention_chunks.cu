@@ -58,8 +58,8 @@ constexpr uint32_t kDiag = kCol + 128;         // the same continued by zeros (r
 constexpr uint32_t kDiagWords = 68;
 constexpr uint32_t kDec = kDiag + 4 * kDiagWords * 4;   // d^0 .. d^128
 constexpr uint32_t kWhole = kDec + 520;                 // d^128 as the factor of whole chunks
-constexpr uint32_t kBars = kWhole + sizeof(SteadyPower);
-static_assert(sizeof(SteadyPower) == 16 && kBars % 8 == 0);
+constexpr uint32_t kBars = kWhole + 16;
+static_assert(sizeof(SteadyPower) <= 16);
 enum Bar {   // [stage], [parity of the chunk], or one
     kFull,                                                // a, b and c are loaded
     kFreeA = kFull + kStages, kFreeB = kFreeA + kStages,  // the last product that reads it is done (without y: and S behind the chunk is known)
@@ -108,6 +108,12 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
 }
 __device__ __forceinline__ float2 unpack2(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 __device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf2(v.x, v.y); }
+// The part in front of others: bf16's largest number, not infinity, for what lies beyond that, which the last part then has.
+__device__ __forceinline__ uint32_t pack2_finite(float2 v) {
+    uint32_t u;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(v.y), "f"(v.x));
+    return u;
+}
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __fadd2_rn(a, make_float2(-b.x, -b.y)); }
 // What is not finite in 16 columns (two pieces) of a token becomes zero, and its place is noted: first + 127 - token (reversed: + token).
 // In loops, as all that is rare or can be: a kernel of several roles lives on what the instruction caches hold of each.  Unrolled, with this for
@@ -324,7 +330,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 s = S[4 * q + e];
-                    hi[e] = pack2(s);
+                    hi[e] = pack2_finite(s);
                     lo[e] = pack2(sub2(s, unpack2(hi[e])));
                 }
                 sts16(base + kS + piece(row, q), make_uint4(hi[0], hi[1], hi[2], hi[3]));
@@ -345,7 +351,7 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
             }
             wait_turn(kAddDone, it);
             tc_fence_after();
-            float dn = tokens_of(it) == kL ? whole.next() : dec[tokens_of(it)];
+            float dn = tokens_of(it) == kL ? whole.factor((uint32_t)it) : dec[tokens_of(it)];
             if (bad_chunk[it % kStages] == it && bad_from[it % kStages * kN + row] >= it * kL) dn = __uint_as_float(0x7fffffffu);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -429,9 +435,9 @@ chunk_kernel(const __grid_constant__ Maps maps, const ChunkArgs p) {
                     for (int e = 0; e < 2; ++e) {
                         const int r = i % 4 * 2 + e;
                         float2 x = __fmul2_rn(unpack2(in[i / 2][i % 2 * 2 + e]), w[i]);
-                        hi[i / 4][r] = pack2(x);
+                        hi[i / 4][r] = pack2_finite(x);
                         x = sub2(x, unpack2(hi[i / 4][r]));
-                        mid[i / 4][r] = pack2(x);
+                        mid[i / 4][r] = pack2_finite(x);
                         lo[i / 4][r] = pack2(sub2(x, unpack2(mid[i / 4][r])));
                     }
                 }

@@ -67,3 +67,41 @@ def test_every_entry_that_is_not_finite_is_found_in_segments(pkg, cuda, dtype, T
     reached = torch.arange(T, device=cuda)[:, None] >= of_column
     assert torch.equal(torch.isfinite(got.output[0, :, 0].float()), ~reached)
     assert not bool(torch.isfinite(got.next_state).any())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 16, 17, 33, 200, 1500])
+def test_infinite_states_stay_infinite(pkg, cuda, T, dtype):
+    """One entry of a state that is infinite: it stays, it makes one row of the outputs and one of the queries' gradient infinite, with
+    the sign that the formula gives them, and nothing else is touched."""
+    x, dy, ds = _inputs(cuda, 2, T, 2, 64, dtype, seed=T)
+    x["log_decay"] = torch.tensor([-0.01, -0.002], device=cuda)
+
+    def call():
+        inputs = pkg.LinearAttentionForwardInputs(x["q"], x["k"], x["v"], x["log_decay"])
+        out = _call(pkg, x)
+        (dq, dk, dv), ds0 = pkg.linear_attention_backward(inputs, dy, ds, initial_state=x["s0"])
+        return out.output.clone(), out.next_state.clone(), dq, dk, dv, ds0
+
+    want = call()
+    inf = float("inf")
+    for row, column, entry in ((5, 9, inf), (7, 3, -inf)):
+        x["s0"][0, 1, row, column] = entry
+        want[1][0, 1, row, column] = entry
+        want[0][0, :, 1, row] = entry * x["q"][0, :, 1, column].float().sign()
+        want[2][0, :, 1, column] = entry * dy[0, :, 1, row].float().sign()
+    for name, a, b in zip(("output", "state", "query", "key", "value", "state gradient"), call(), want):
+        assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("T", [60, 200])
+def test_states_beyond_the_largest_bf16_number(pkg, cuda, T):
+    """fp32 goes on for half a step of bf16 behind bf16's largest number."""
+    x = _inputs(cuda, 1, T, 2, 64, BF16)[0]
+    x["s0"][0, 1, 5, 9], x["s0"][0, 1, 7, 3] = 3.4e38, -3.4e38
+    x["log_decay"] = torch.tensor([-0.01, -0.002], device=cuda)
+    out = _call(pkg, x)
+    y, s = ref.attention(**x)
+    my, ms = ref.attention(**_abs(x))
+    _close(out.output, y, my, T, 64, BF16, "output")
+    _close(out.next_state, s, ms, T, 64, BF16, "state")
