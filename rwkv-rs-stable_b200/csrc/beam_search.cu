@@ -63,6 +63,8 @@ __device__ C block_first(C c, C *shared) {
 constexpr int kVectors = 4;                          // 16-byte vectors a thread has in registers, and as many on their way
 constexpr int kMostAside = kThreads + 32;            // threads' vectors put aside: gone through when there are more than 32
 constexpr int kMostKept = 2048;                      // logits over the bound: room for; it is raised when they are many for K
+constexpr int kMostRanked = 256;                     // of them, each against each; more come of many equal ones alone
+constexpr float kLowest = -1e38f;                    // where x log2 e is still a number; masks are below
 constexpr int kMostSplits = 32;                      // CTAs on a row
 
 // Pieces of a row.  They start on 16 bytes, the first at or (where rows are not whole vectors) before the row's start.
@@ -79,22 +81,24 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u ^ ((u & 0x80000000u) ? 0x80000000u : 0xffffffffu)); }
 
 // The lanes' values in falling order.
-__device__ __forceinline__ uint32_t warp_sort(uint32_t x, int lane) {
+template <typename U>
+__device__ __forceinline__ U warp_sort(U x, int lane) {
 #pragma unroll
     for (int k = 2; k <= 32; k *= 2)
 #pragma unroll
         for (int j = k / 2; j > 0; j /= 2) {
-            const uint32_t y = __shfl_xor_sync(0xffffffffu, x, j);
+            const U y = __shfl_xor_sync(0xffffffffu, x, j);
             x = ((lane & j) == 0) == ((lane & k) == 0) ? max(x, y) : min(x, y);
         }
     return x;
 }
 // The 32 largest of two falling lists, falling.
-__device__ __forceinline__ uint32_t warp_merge(uint32_t x, uint32_t other, int lane) {
+template <typename U>
+__device__ __forceinline__ U warp_merge(U x, U other, int lane) {
     x = max(x, __shfl_sync(0xffffffffu, other, 31 - lane));
 #pragma unroll
     for (int j = 16; j > 0; j /= 2) {
-        const uint32_t y = __shfl_xor_sync(0xffffffffu, x, j);
+        const U y = __shfl_xor_sync(0xffffffffu, x, j);
         x = (lane & j) == 0 ? max(x, y) : min(x, y);
     }
     return x;
@@ -108,16 +112,17 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
     constexpr float kLog2e = 1.4426950408889634f;
     __shared__ Candidate<float, int> shared[kWarps];
     __shared__ uint32_t tops[kWarps][32];
+    __shared__ uint64_t firsts[kWarps][32];
     __shared__ float2 partial[kWarps];
     __shared__ uint64_t kept[kMostKept];
     __shared__ uint64_t best[32];
     __shared__ uint4 aside[kMostAside][kVectors];
     __shared__ int aside_from[kMostAside];   // its first token
-    __shared__ int n_kept, n_aside, full[2];   // `full`, of even and odd pieces: what is aside is to be gone through
+    __shared__ int n_kept, n_before, n_aside, full[2];   // `full`, of even and odd pieces: what is aside is to be gone through
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t out = blockIdx.x, row = out / splits;
     const int split = (int)(out - row * splits), stop = min(n_pieces, (split + 1) * each);
-    if (tid == 0) n_kept = n_aside = full[0] = full[1] = 0;
+    if (tid == 0) n_kept = n_before = n_aside = full[0] = full[1] = 0;
     wait_for_previous();
     let_next_in();
     const T *logits = static_cast<const T *>(p.logits);
@@ -161,26 +166,48 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
         else return __uint_as_float(j & 1 ? w[j % 8 / 2] & 0xffff0000u : w[j % 8 / 2] << 16);
     };
     auto token = [&](int lead, int j) { return lead + (j / VEC * kThreads + tid) * VEC + j % VEC; };
-    float bound = -INFINITY, top = -INFINITY, sum = 0.f;   // the last two of this thread's logits
-    bool slow = false;
+    float top = -INFINITY, sum = 0.f;   // of this thread's logits
+    // What is looked at reaches this (-inf never does).  Where K tokens in front of the piece were kept it is above the least of them: of equals they
+    // go first.
+    float bound = -FLT_MAX;
     // All threads: what is aside and reaches the bound is kept; with much kept the bound is raised.  (Nobody puts aside meanwhile.)
     auto go_through = [&] {
         __syncthreads();
         const int n = n_aside * kPer;
-        for (int i = tid; i < n; i += kThreads) {
-            const int e = i / kPer, j = i % kPer;
-            const float x = ldf(reinterpret_cast<const T *>(aside[e]) + j);
-            if (x >= bound && x > -INFINITY) {
-                const int at = atomicAdd(&n_kept, 1);
+        auto each_aside = [&](auto &&use) {
+            for (int i = tid; i < n; i += kThreads) {
+                const int e = i / kPer, j = i % kPer;
+                const float x = ldf(reinterpret_cast<const T *>(aside[e]) + j);
                 // (-0 is 0)
-                if (at < kMostKept) kept[at] = (uint64_t)ordered(x + 0.f) << 32 | (uint32_t)~(uint32_t)(aside_from[e] + j / VEC * kThreads * VEC + j % VEC);
+                if (x >= bound) use((uint64_t)ordered(x + 0.f) << 32 | (uint32_t)~(uint32_t)(aside_from[e] + j / VEC * kThreads * VEC + j % VEC));
             }
+        };
+        auto keep = [&](uint64_t least, int enough) {
+            each_aside([&](uint64_t x) {
+                if (x < least || *(volatile int *)&n_kept > enough) return;
+                const int at = atomicAdd(&n_kept, 1);
+                if (at < kMostKept) kept[at] = x;
+            });
+            __syncthreads();
+        };
+        keep(0, kMostRanked);
+        const bool many = n_kept > kMostRanked;
+        if (many) {
+            // Again, by the K-th of what is the threads' first: K threads at most have any that reach it, 36 each.
+            uint64_t mine = 0;
+            each_aside([&](uint64_t x) { mine = max(mine, x); });
+            firsts[warp][lane] = warp_sort(mine, lane);
+            __syncthreads();
+            if (tid == 0) n_kept = n_before;
+            uint64_t list = firsts[0][lane];
+#pragma unroll 1
+            for (int w = 1; w < kWarps; ++w) list = warp_merge(list, firsts[w][lane], lane);
+            __syncthreads();
+            keep(__shfl_sync(0xffffffffu, list, p.K - 1), kMostKept);
         }
-        __syncthreads();
         if (tid == 0) n_aside = 0;
-        if (n_kept > 2 * p.K + 16) {
-            const int n = min(n_kept, kMostKept);
-            slow = slow || n_kept > kMostKept;
+        if (many || n_kept > 2 * p.K + 16) {   // (there are K)
+            const int n = n_kept;
             for (int i = tid; i < n; i += kThreads) {
                 const uint64_t mine = kept[i];
                 int rank = 0;
@@ -190,9 +217,10 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
             __syncthreads();
             if (tid < p.K) kept[tid] = best[tid];
             if (tid == 0) n_kept = p.K;
-            bound = fmaxf(bound, unordered((uint32_t)(best[p.K - 1] >> 32)));
+            bound = fmaxf(bound, unordered((uint32_t)(best[p.K - 1] >> 32) + 1));
         }
         __syncthreads();
+        if (tid == 0) n_before = n_kept;
     };
     auto sum_of_block = [&](float x) {
 #pragma unroll
@@ -224,12 +252,13 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
             for (int j = 1; j < kPer / 2; ++j) m = __hmax2(m, h[j]);
             most = fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
         }
-        // 2^(x log2 e - c), c being the maximum's log2 e rounded; what the rounding takes is put back behind the sum
+        // 2^(x log2 e - c), c being the maximum's log2 e rounded; what the rounding takes is put back behind the sum.  (A thread that has seen nothing
+        // but masked logits has no sum: beside any other it is nothing, and a row without any other is summed below.)
         if (most > top) {
             sum *= exp2f((top - most) * kLog2e);
             top = most;
         }
-        if (top > -INFINITY) {
+        if (top > kLowest) {
             const float c = top * kLog2e;
             float2 part = make_float2(0.f, 0.f);
 #pragma unroll
@@ -255,7 +284,7 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
             go_through();
             if (tid == 0) full[(piece + 1) & 1] = 0;
         }
-        if (most >= bound && most > -INFINITY) {
+        if (most >= bound) {
             const int at = atomicAdd(&n_aside, 1);
 #pragma unroll
             for (int i = 0; i < NV; ++i) aside[at][i] = raw[i];
@@ -282,11 +311,24 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
         if (tid == 0) sums[out] = make_float2(-INFINITY, 0.f);
         return;
     }
-    const float total = sum_of_block(top == -INFINITY ? sum : sum * exp2f((top - block_top) * kLog2e));
-    const int n = n_kept;
-    // (too few above -inf; a flood of equal ones; NaN, infinities and numbers near them, which the sum does not stand)
-    if (n >= p.K && n <= kMostKept && !slow && total < INFINITY && fabsf(block_top) < 1e38f) {
-        if (tid == 0) sums[out] = make_float2(block_top, total);
+    float total = sum_of_block(top == -INFINITY ? sum : sum * exp2f((top - block_top) * kLog2e));
+    // (NaN, +inf and numbers near it, which the sum does not stand)
+    const bool plain = total < INFINITY && block_top < -kLowest;
+    const float top_clean = clean(block_top);
+    // Summed again, which is rare: NaN and +inf as what they count for; a row of masks alone; and a row of fewer logits than are chosen, whose terms are
+    // the same numbers whichever thread has them, so that equal rows are equal wherever they lie.
+    if (!plain || block_top <= kLowest || (n_pieces == 1 && n_kept < p.K)) {
+        sum = 0.f;
+        for (int piece = split * each; piece < stop; ++piece) {
+            load(raw, base + (int64_t)piece * kPiece);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) sum += expf(clean(value(j)) - top_clean);
+        }
+        total = sum_of_block(sum);
+    }
+    if (tid == 0) sums[out] = make_float2(top_clean, total);
+    if (plain) {
+        const int n = n_kept;
         for (int i = tid; i < n; i += kThreads) {
             const uint64_t mine = kept[i];
             int rank = 0;
@@ -296,18 +338,19 @@ beam_rows_kernel(const BeamSelectArgs p, int splits, int each, int n_pieces, flo
                 tokens[out * p.K + rank] = (int)~(uint32_t)mine;
             }
         }
+        if (n < p.K && warp == 0) {   // all that is above -inf was kept: the first other tokens fill up
+            bool other = from + lane < to;
+            for (int j = 0; j < n; ++j) other = other && (int)~(uint32_t)kept[j] != from + lane;
+            const uint32_t others = __ballot_sync(0xffffffffu, other);
+            const int rank = n + (other ? __popc(others & ((1u << lane) - 1)) : __popc(others) + __popc(~others & ((1u << lane) - 1)));
+            if (rank < p.K) {
+                values[out * p.K + rank] = -INFINITY;
+                tokens[out * p.K + rank] = other ? from + lane : -1;
+            }
+        }
         return;
     }
-    // The slow way, for what is rare: one after the other, with NaN and +inf as what they count for.
-    const float top_clean = clean(block_top);
-    sum = 0.f;
-    for (int piece = split * each; piece < stop; ++piece) {
-        load(raw, base + (int64_t)piece * kPiece);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) sum += expf(clean(value(j)) - top_clean);
-    }
-    sum = sum_of_block(sum);
-    if (tid == 0) sums[out] = make_float2(top_clean, sum);
+    // NaN and the like: one choice after the other.
     Candidate<float, int> last{INFINITY, -1};
     for (int k = 0; k < p.K; ++k) {
         Candidate<float, int> found{-INFINITY, INT_MAX};
