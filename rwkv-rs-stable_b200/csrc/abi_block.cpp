@@ -482,12 +482,14 @@ int rwkv7_beam_reorder(const rwkv7_tensor *const *states, int32_t n, const rwkv7
     if (guard.error() != cudaSuccess) return cuda_fail("cudaSetDevice", (int)guard.error());
     RWKV7_TRY(num_sms(parents_t->device, &p.num_sms));
     if (int e = device_status_ptr(parents_t->device, &p.status)) return cuda_fail("device status word", e);
-    for (int i = 0; i < n; ++i) {
-        const int64_t row = (int64_t)(bytes_of(states[i]) / (size_t)(B * I));
-        if (row > 0) p.tensors[p.n++] = {states[i]->data, out == nullptr ? states[i]->data : out[i]->data, row};
-        if (p.n == kMaxReordered || (i == n - 1 && p.n > 0)) {
-            if (int e = launch_beam_reorder(p, (cudaStream_t)stream)) return cuda_fail("beam_reorder launch", e);
-            p.n = 0;
+    for (const int unit : kReorderUnits) {
+        for (int i = 0; i < n; ++i) {
+            const int64_t row = (int64_t)(bytes_of(states[i]) / (size_t)(B * I));
+            if (row > 0 && beam_reorder_unit(row) == unit) p.tensors[p.n++] = {states[i]->data, out == nullptr ? states[i]->data : out[i]->data, row};
+            if (p.n == kMaxReordered || (i == n - 1 && p.n > 0)) {
+                if (int e = launch_beam_reorder(p, unit, (cudaStream_t)stream)) return cuda_fail("beam_reorder launch", e);
+                p.n = 0;
+            }
         }
     }
     return RWKV7_OK;

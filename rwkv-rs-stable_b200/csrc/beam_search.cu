@@ -595,13 +595,9 @@ int launch_beam_select(const BeamSelectArgs &p, void *workspace, size_t workspac
                                   (const float *)values, (const int *)tokens);
 }
 
-int launch_beam_reorder(const BeamReorderArgs &p, cudaStream_t stream) {
-    int64_t unit = 16, most = 0;
-    for (int i = 0; i < p.n; ++i) {
-        while (p.tensors[i].row_bytes % unit != 0) unit /= 2;
-        if (p.tensors[i].row_bytes > most) most = p.tensors[i].row_bytes;
-    }
-    if (unit == 8) unit = 4;
+int launch_beam_reorder(const BeamReorderArgs &p, int unit, cudaStream_t stream) {
+    int64_t most = 0;
+    for (int i = 0; i < p.n; ++i) most = std::max(most, p.tensors[i].row_bytes);
     const unsigned blocks = (unsigned)std::min<int64_t>((p.B * (most / unit) + kThreads - 1) / kThreads, (int64_t)p.num_sms * 8);
     if (unit == 16) return (int)launch_reorder<uint4>(p, blocks, stream);
     if (unit == 4) return (int)launch_reorder<uint32_t>(p, blocks, stream);

@@ -283,7 +283,11 @@ struct BeamSelectArgs {
 size_t beam_select_workspace_bytes(const BeamSelectArgs &p);
 size_t beam_select_min_workspace_bytes(const BeamSelectArgs &p);
 int launch_beam_select(const BeamSelectArgs &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
-constexpr int kMaxReordered = 48;   // tensors per launch
+constexpr int kMaxReordered = 48;   // tensors per launch: two of each of 24 layers; they take 1152 of its 4096 bytes of parameters
+// Bytes that a thread moves at once, the same for all tensors of a launch: beside states of 134 MB one row of 8 bytes would make 89 us of 47, one of
+// 6 bytes 159, so these have launches of their own.
+constexpr int kReorderUnits[] = {16, 4, 2};
+constexpr int beam_reorder_unit(int64_t row_bytes) { return row_bytes % 16 == 0 ? 16 : row_bytes % 4 == 0 ? 4 : 2; }
 struct BeamReorderArgs {
     struct Item {
         const void *from;   // B*I rows
@@ -298,6 +302,6 @@ struct BeamReorderArgs {
     int *status;
     int num_sms;
 };
-int launch_beam_reorder(const BeamReorderArgs &p, cudaStream_t stream);
+int launch_beam_reorder(const BeamReorderArgs &p, int unit, cudaStream_t stream);
 
 }  // namespace rwkv7
