@@ -105,3 +105,61 @@ def test_states_beyond_the_largest_bf16_number(pkg, cuda, T):
     my, ms = ref.attention(**_abs(x))
     _close(out.output, y, my, T, 64, BF16, "output")
     _close(out.next_state, s, ms, T, 64, BF16, "state")
+
+
+@pytest.mark.parametrize("T,pieces", [(200, "one"), (1500, "segments")])
+def test_a_state_keeps_all_bits_of_its_terms(pkg, cuda, T, pieces):
+    """One token has a value, so the state is one product: nothing is added that could hide what its parts leave out.  Its decay is taken as two
+    powers at most, with exponents down to -2: each within 4 half steps (expf) and the rounding of its exponent, 2 more; the product with the
+    value, the three sums of its parts and the state's own scalings add a half step or (a sum on the tensor cores) two each."""
+    H = 32 if pieces == "one" else 4
+    x = _inputs(cuda, 5, T, H, 64, BF16, state=False, seed=6)[0]
+    x["log_decay"] = -(2.0 / T) * torch.rand(H, generator=torch.Generator().manual_seed(1)).to(cuda)
+    at = torch.randint(0, T, (5, H), generator=torch.Generator().manual_seed(2)).to(cuda)
+    only = torch.arange(T, device=cuda)[None, :, None] == at[:, None]
+    x["v"] = torch.where(only[..., None], x["v"], torch.zeros_like(x["v"]))
+    got = _call(pkg, x).next_state.double()
+    v, k = (x[n].double()[only.nonzero(as_tuple=True)].view(-1, 64) for n in "vk")
+    where = only.nonzero()
+    want = torch.empty_like(got)
+    power = torch.exp(x["log_decay"].double()[where[:, 2]] * (T - 1 - where[:, 1]))
+    want[where[:, 0], where[:, 2]] = power[:, None, None] * v[:, :, None] * k[:, None, :]
+    scalings = T // 128 + 1
+    off = ((got - want).abs() / want.abs().clamp_min(1e-30)).max() / ref.U
+    # (without the last eight bits of a weighted value: up to 64)
+    assert float(off) <= 2 * 6 + 1 + 3 * 2 + 3 * scalings, float(off)
+
+
+def test_a_carried_state_enters_the_outputs_with_sixteen_bits(pkg, cuda):
+    """A query of one component and no values: an output is one entry of the state and its decay, rounded to bf16 once, with what the state's
+    two bf16 parts (2^-17 of it) and fp32 (16 half steps) leave out before that."""
+    T = 100
+    x = _inputs(cuda, 2, T, 40, 64, BF16, seed=9)[0]
+    x["v"].zero_()
+    one = torch.randint(0, 64, (2, T, 40), generator=torch.Generator().manual_seed(3)).to(cuda)
+    x["q"] = torch.nn.functional.one_hot(one, 64).bfloat16()
+    got = _call(pkg, x).output.double()
+    picked = x["s0"].double().transpose(-1, -2)[torch.arange(2, device=cuda)[:, None, None], torch.arange(40, device=cuda), one]   # B T H N
+    want = picked * torch.exp(x["log_decay"].double() * (torch.arange(T, device=cuda)[:, None] + 1))[None, ..., None]
+    half = torch.exp2(torch.floor(torch.log2(want.abs().clamp_min(1e-300)))) * 2.0 ** -8   # of a step of bf16 there
+    # (by the first part alone 2^-9 more)
+    assert bool(((got - want).abs() <= half * (1 + 2.0 ** -7) + (2.0 ** -17 + 16 * ref.U) * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N", [32, 128])
+def test_padded_batches_of_other_head_sizes_in_segments(pkg, cuda, N, dtype):
+    lens = [700, 0, 333]
+    x, dy, ds = _inputs(cuda, 3, 700, 2, N, dtype, lens=lens, seed=N)
+    for b, e in enumerate(lens):
+        for t in (x["q"], x["k"], x["v"], dy):
+            t[b, e:] = float("nan")
+    assert pkg.linear_attention_workspace_bytes(3, 700, 2, N, dtype) > 0   # (there are segments)
+    out = _call(pkg, x)
+    inputs = pkg.LinearAttentionForwardInputs(x["q"], x["k"], x["v"], x["log_decay"], context_lens=x["lens"])
+    grads, ds0 = pkg.linear_attention_backward(inputs, dy, ds, initial_state=x["s0"])
+    dy0 = torch.nan_to_num(dy, nan=0.0)
+    wants = [*ref.attention(**x), *ref.attention_grads(**x, dy=dy0, ds=ds)]
+    mags = [*ref.attention(**_abs(x)), *ref.attention_grads(**_abs(x), dy=dy0.abs(), ds=ds.abs())]
+    for name, got, w, m in zip(("output", "state", "query", "key", "value", "state gradient"), (out.output, out.next_state, *grads, ds0), wants, mags):
+        _close(got, w, m, 700, N, dtype, name)

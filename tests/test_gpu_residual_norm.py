@@ -273,3 +273,23 @@ def test_captured_and_replayed_with_new_values(pkg, cuda):
     torch.cuda.synchronize()
     assert torch.equal(out.next_residual, want.next_residual) and torch.equal(out.normed, want.normed)
     assert all(torch.equal(a, b) for a, b in zip(back, want_back))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_autograd_of_strided_and_broadcast_inputs(pkg, cuda, dtype):
+    """A gate that all rows share, a block output out of a larger projection, parameters out of one tensor: the autograd form lays them out, and
+    the gradients come back in the places they were taken from."""
+    B, T, C = 2, 5, 96
+    t, grads = _inputs(cuda, B, T, C, dtype, FULL, seed=5)
+    want_in = dict(t, gate=t["gate"][:1, :1].expand(B, T, C).contiguous())
+    want = dict(zip(NAMES, pkg.residual_norm_backward(pkg.ResidualNormForwardInputs(**want_in), *grads)))
+    gate = t["gate"][:1, :1].clone().requires_grad_()
+    wide = torch.stack([t["block_output"], t["residual"]], dim=2).requires_grad_()
+    params = torch.stack([t[n] for n in NAMES[3:]], dim=1).requires_grad_()
+    strided = dict(zip(NAMES[3:], params.unbind(1)), residual=t["residual"].transpose(0, 1).contiguous().transpose(0, 1), block_output=wide[:, :, 0],
+                   gate=gate.expand(B, T, C))
+    x, z = pkg.residual_norm_autograd(pkg.ResidualNormForwardInputs(**strided))
+    of_gate, of_wide, of_params = torch.autograd.grad((x, z), (gate, wide, params), grads)
+    assert torch.equal(of_wide[:, :, 0], want["block_output"]) and bool((of_wide[:, :, 1] == 0).all())
+    assert all(torch.equal(of_params[:, i], want[n]) for i, n in enumerate(NAMES[3:]))
+    assert torch.equal(of_gate, want["gate"].sum((0, 1), keepdim=True))
