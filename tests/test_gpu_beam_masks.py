@@ -32,13 +32,21 @@ def _allowed(cuda, B, I, kind):
 
 
 def _time(call):
-    for _ in range(3):
+    """Milliseconds on the device, of four calls in a graph (a busy host counts for nothing)."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
         call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(4):
+            call()
     times = []
     for _ in range(7):
         ends = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
         ends[0].record()
-        call()
+        graph.replay()
         ends[1].record()
         torch.cuda.synchronize()
         times.append(ends[0].elapsed_time(ends[1]))
