@@ -16,7 +16,8 @@
 //
 // S is in registers: a thread holds four rows x 16 columns, the columns in groups of four that alternate between the threads of a
 // row, so that these read neighbouring pieces.  A token then costs 64 multiply-adds for nine loads from shared memory; one row a
-// thread needed sixteen for 32.  For one token it is bound by the bytes of S (512 sequences of 40 heads 112 us, 6.1 TB/s); for many by the chain of a
+// thread needed sixteen for 32.  For one token it is bound by the bytes of S (512 sequences of 40 heads 112 us, 6.1 TB/s, into a state
+// that is there, 119 with its allocation); for many by the chain of a
 // block, 5.3 us at N = 64 on two warps, which several CTAs an SM overlap (2 x 1000 tokens of 12 heads in fp32 43 us, three launches of
 // segments of two blocks).
 #include <cuda_bf16.h>
@@ -41,7 +42,7 @@ struct Shape {
     static constexpr int kThreads = N / kRows * kShare;
     static constexpr int kPitch = N + 4;                           // floats of a staged row
     // CTAs an SM is to hold, which spills a few of 160 registers: one token of 512 sequences of 40 heads 118 -> 112 us, 4 x 1000 fp32 tokens of 32
-    // heads 177 -> 157, N = 128 of 16 heads 397 -> 308.  The pass that only adds to states spills more than it gains at N = 64.
+    // heads 177 -> 157, N = 128 of 16 heads 397 -> 308 (313 with what came since).  The pass that only adds to states spills more than it gains at N = 64.
     static constexpr int resident(bool adds) { return N == 128 ? 2 : N == 64 ? (adds ? 1 : 8) : 16; }
 };
 

@@ -23,7 +23,8 @@
 // for its sum, its sum for w C, y for P's decays, and each of these hands over through a barrier.
 //
 // Precision: y is rounded to bf16, and so is P (once); S stays in fp32 registers and enters Y2 as hi + lo (16 bits and a
-// sign), because its errors would add up; the sum for S' takes w C as hi + mid + lo, all 24 bits, because S is an fp32 output.
+// sign), because its errors would add up; the sum for S' takes w C as hi + mid + lo, all 24 bits, because S is an fp32 output.  The decays inside
+// a chunk are fp32 powers (expf); d^128, which a state meets again with every chunk, comes from 64 bits.
 //
 // Entries of c that are not finite would reach tokens on the other side of the mask (0 x inf): a chunk that has some takes
 // them as zero and sets what they do reach, the column's later tokens and the state's column, to NaN.
