@@ -543,9 +543,10 @@ int rwkv7_lm_head_ce_finalize(const rwkv7_tensor *partials_all, const rwkv7_tens
  * ones as T): the tokens behind it are not read into anything, their output is zero, and the final state is the one at the length.
  * BF16 with N = 64, from 17 (with many chains 48) tokens on, rounds the products query . key between tokens of a chunk to bf16 once, and
  * takes 16 bits and a sign of a carried state into an output; states are summed from all 24 bits.
- * An infinite entry of a state stays what it is and makes infinite what the formula says.  An entry of query, key or value that is not
- * finite makes what it reaches (a key its column of the state and the outputs from its token on, a value its row of both, a query its
- * token's output) not finite, an infinity or NaN, and nothing else.
+ * An infinite entry of a state stays what it is and makes infinite what the formula says while exp(len_b log_decay) is a normal fp32
+ * number; beyond that it may become NaN.  An entry of query, key or value that is not finite makes what it reaches (a key its column of
+ * the state and the outputs from its token on, a value its row of both, a query its token's output) not finite, an infinity or NaN, and
+ * nothing else.
  * The workspace lets a call of few chains work on several parts of a sequence at once; a smaller one than the call below names, or
  * NULL, makes fewer parts of it (results differ in the last bits).  It must start on 16 bytes.
  */

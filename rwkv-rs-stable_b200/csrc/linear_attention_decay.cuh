@@ -8,8 +8,9 @@
 
 namespace rwkv7 {
 
-// The rounded power, taken 256 times over a long memory, would be off 256 times the same way (1.6e-5 of a state, 3e-8 a chunk).  So it is rounded
-// now down, now up, each as often as the power lies near it: the product of any number of factors in a row is off by one step of one factor.
+// The rounded power, taken 256 times over a long memory, would be off 256 times the same way (by up to 3e-8 of a state, and as expf gives it by more:
+// 1.6e-5 after 256 chunks).  So it is rounded now down, now up, each as often as the power lies near it: the product of any number of factors in a row
+// is off by one step of one factor.
 // (The part that rounding took could be multiplied as well, at an instruction more for each two elements, and as 0 x inf or inf - inf it would make
 // an infinite element NaN.)  Nothing is carried from factor to factor but their number, so that it may stand in shared memory.
 struct SteadyPower {

@@ -163,3 +163,52 @@ def test_padded_batches_of_other_head_sizes_in_segments(pkg, cuda, N, dtype):
     mags = [*ref.attention(**_abs(x)), *ref.attention_grads(**_abs(x), dy=dy0.abs(), ds=ds.abs())]
     for name, got, w, m in zip(("output", "state", "query", "key", "value", "state gradient"), (out.output, out.next_state, *grads, ds0), wants, mags):
         _close(got, w, m, 700, N, dtype, name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 33, 200, 1500])
+def test_infinite_gradients_of_the_final_state_stay_infinite(pkg, cuda, T, dtype):
+    x, dy, ds = _inputs(cuda, 2, T, 2, 64, dtype, seed=T)
+    x["log_decay"] = torch.tensor([-0.01, -0.002], device=cuda)
+
+    def call():
+        (dq, dk, dv), ds0 = pkg.linear_attention_backward(pkg.LinearAttentionForwardInputs(x["q"], x["k"], x["v"], x["log_decay"]), dy, ds,
+                                                          initial_state=x["s0"])
+        return dq, dk, dv, ds0
+
+    want = call()
+    inf = float("inf")
+    for row, column, entry in ((5, 9, inf), (7, 3, -inf)):
+        ds[1, 0, row, column] = entry
+        want[3][1, 0, row, column] = entry
+        want[2][1, :, 0, row] = entry * x["k"][1, :, 0, column].float().sign()
+        want[1][1, :, 0, column] = entry * x["v"][1, :, 0, row].float().sign()
+    for name, a, b in zip(("query", "key", "value", "state gradient"), call(), want):
+        assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 40, 200, 1500])
+def test_what_is_not_finite_reaches_its_own(pkg, cuda, T, dtype):
+    """One key, then one query, of a head: columns of the state, outputs from that token on or of that token; everything else as without it."""
+    x = _inputs(cuda, 2, T, 2, 64, dtype, seed=T + 1)[0]
+    x["log_decay"] = torch.tensor([-0.01, -0.002], device=cuda)
+    clean = _call(pkg, x)
+    t = T // 2
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        k = x["k"].clone()
+        k[1, t, 0, 11] = bad
+        out = _call(pkg, dict(x, k=k))
+        reached = torch.zeros_like(out.output, dtype=torch.bool)
+        reached[1, t:, 0] = True
+        assert torch.equal(torch.isfinite(out.output), ~reached) and torch.equal(out.output[~reached], clean.output[~reached])
+        column = torch.zeros_like(out.next_state, dtype=torch.bool)
+        column[1, 0, :, 11] = True
+        assert torch.equal(torch.isfinite(out.next_state), ~column) and torch.equal(out.next_state[~column], clean.next_state[~column])
+        q = x["q"].clone()
+        q[1, t, 0, 11] = bad
+        out = _call(pkg, dict(x, q=q))
+        reached = torch.zeros_like(out.output, dtype=torch.bool)
+        reached[1, t, 0] = True
+        assert torch.equal(torch.isfinite(out.output), ~reached) and torch.equal(out.output[~reached], clean.output[~reached])
+        assert torch.equal(out.next_state, clean.next_state)
